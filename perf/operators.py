@@ -12,7 +12,7 @@ The operators (``own``: as the framework's entry points; otherwise plain):
 
 The 8-bit pages: a block is 16 tokens of one key/value head.  Keys [pages, heads, page, size], values transposed within a
 block [pages, heads, page / 16, size, 16]; per block a scale 2^e with the smallest e for which the block's largest
-magnitude is at most 448 (e4m3) or 127 (int8) times 2^e, e within [-100, 100].  A block that grows keeps or raises its
+magnitude is at most 448 (e4m3) or 127 (int8) times 2^e, e within [-40, 40].  A block that grows keeps or raises its
 scale; what it holds is then encoded again.  Keys are rounded to bfloat16 before they are encoded.
 """
 from __future__ import annotations
@@ -26,7 +26,7 @@ import torch
 own = False
 
 BLOCK = 16
-E_MIN, E_MAX = -100, 100
+E_MIN, E_MAX = -40, 40
 EPS = 1e-6
 THETA = 1e6
 VOCAB = 151936
