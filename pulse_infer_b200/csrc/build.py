@@ -30,10 +30,13 @@ SOURCES = {
     "gemm_tcgen05": "gemm_tcgen05.cu",
     "attention_simple": "attention_simple.cu",
     "sampling": "sampling.cu",
+    "page_maps": "page_maps.cu",
+    "cache_8bit": "cache_8bit.cu",
+    "attention_8bit": "attention_8bit.cu",
 }
 ATTENTION_MMA_SOURCE = "attention_mma.cu"
 ATTENTION_TCGEN05_SOURCE = "attention_tcgen05.cu"
-HEADERS = ["common.cuh", "attention_noalloc.h"]
+HEADERS = ["common.cuh", "attention_noalloc.h", "cache_8bit.cuh"]
 
 _lock = threading.Lock()
 

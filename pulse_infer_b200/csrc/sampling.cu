@@ -1,6 +1,7 @@
 // Token selection on the device from 32-bit logits: greedy (argmax) and temperature sampling with
 // optional top-k and top-p, one thread block per row, plus a small kernel that edits single logits
-// (presence penalty, banned ids).
+// (presence penalty, banned ids) and one that applies all rules of a request to its row in one pass
+// (penalties over the token history, biases, a mask of allowed ids).
 //
 // Reference parity (the reference samples on the CPU):
 //   greedy       src/scheduler/continuous_batch_engine.cpp:20-62   strict '>' so the lowest index wins ties
@@ -339,4 +340,128 @@ PI_EXPORT int pi_logit_edit(float* logits, int ld, int vocab, const int* rows, c
     if (n <= 0) return 0;
     pi_launch(logit_edit_kernel, dim3((n + 127) / 128), dim3(128), 0, stream, logits, ld, vocab, rows, tokens, values, n, set);
     return pi_check_launch("pi_logit_edit");
+}
+
+// ---------------------------------------------------------------------------------------------------
+// The rules of each row on its logits, in one pass.  With the row's history h (its first prompt_len entries the prompt),
+// seen = v occurs in h, count = occurrences behind the prompt, for every token id v
+//   x = seen ? (x > 0 ? x / repetition : x * repetition) : x
+//   x = x - frequency * count - (seen ? presence : 0) + bias[v],   x = -inf where the row's mask has a zero bit
+// Of several biases of a row for one id the last counts; ids outside the vocabulary are passed over.
+//
+// The logits are read and written once (4 + 4 bytes each: what bounds a large step); a step of one row is bound by latency.
+// A block owns RULE_SLICE ids of a row: it requests its logits, marks the history's ids of its slice in shared memory
+// (every block of the row walks the whole history, 4 bytes an entry out of L2; integer atomics, so the order does not
+// matter), and applies the rules as it stores.  No workspace, no second launch.
+// ---------------------------------------------------------------------------------------------------
+#define RULE_THREADS 256
+#define RULE_SLICE 4096
+#define RULE_VECS (RULE_SLICE / 4 / RULE_THREADS)
+
+struct RuleParams {
+    const float* logits; long long ld; float* out; long long out_ld; int vocab, vec;
+    const int* history; const int* history_off; int history_total; const int* prompt_len;
+    const float* repetition; const float* frequency; const float* presence;
+    const int* bias_off; const int* bias_tokens; const float* bias_values; int bias_total;
+    const unsigned* mask; int mask_rows, mask_words; const int* mask_row;
+};
+
+template <bool BIAS>
+__global__ void __launch_bounds__(RULE_THREADS) logit_rules_kernel(const RuleParams p) {
+    __shared__ unsigned mark[RULE_SLICE];                      // bit 31: in the prompt; below: count behind it
+    __shared__ int bias_at[BIAS ? RULE_SLICE : 1];             // index + 1 of the last bias for the id
+    pdl_wait();
+    pdl_trigger();
+    const int row = blockIdx.y, begin = blockIdx.x * RULE_SLICE, n = min(RULE_SLICE, p.vocab - begin);
+    const float* x = p.logits + (size_t)row * p.ld + begin;
+    float* y = p.out + (size_t)row * p.out_ld + begin;
+    float4 v[RULE_VECS];
+#pragma unroll
+    for (int k = 0; k < RULE_VECS; ++k) {
+        const int i = 4 * (k * RULE_THREADS + threadIdx.x);
+        if (p.vec && i + 4 <= n) {
+            v[k] = *reinterpret_cast<const float4*>(x + i);
+        } else {
+            v[k].x = i < n ? x[i] : 0.0f; v[k].y = i + 1 < n ? x[i + 1] : 0.0f;
+            v[k].z = i + 2 < n ? x[i + 2] : 0.0f; v[k].w = i + 3 < n ? x[i + 3] : 0.0f;
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < RULE_VECS; ++k) {
+        const int i = k * RULE_THREADS + threadIdx.x;
+        reinterpret_cast<uint4*>(mark)[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (BIAS) reinterpret_cast<int4*>(bias_at)[i] = make_int4(0, 0, 0, 0);
+    }
+    __syncthreads();
+    {
+        const int h0 = max(0, min(p.history_off[row], p.history_total)), h1 = max(h0, min(p.history_off[row + 1], p.history_total));
+        const long long gen = (long long)h0 + p.prompt_len[row];
+        for (int h = h0 + threadIdx.x; h < h1; h += RULE_THREADS) {
+            const unsigned at = (unsigned)p.history[h] - (unsigned)begin;
+            if (at < (unsigned)n) {
+                if (h >= gen) atomicAdd(&mark[at], 1u); else atomicOr(&mark[at], 0x80000000u);
+            }
+        }
+    }
+    if (BIAS) {
+        const int b0 = max(0, min(p.bias_off[row], p.bias_total)), b1 = max(b0, min(p.bias_off[row + 1], p.bias_total));
+        for (int b = b0 + threadIdx.x; b < b1; b += RULE_THREADS) {
+            const unsigned at = (unsigned)p.bias_tokens[b] - (unsigned)begin;
+            if (at < (unsigned)n) atomicMax(&bias_at[at], b + 1);
+        }
+    }
+    __syncthreads();
+    const float rep = p.repetition[row], freq = p.frequency[row], pres = p.presence[row];
+    int mrow = p.mask != nullptr ? p.mask_row[row] : -1;
+    if (mrow >= p.mask_rows) mrow = -1;
+    const unsigned* words = mrow >= 0 ? p.mask + (size_t)mrow * p.mask_words + begin / 32 : nullptr;
+#pragma unroll
+    for (int k = 0; k < RULE_VECS; ++k) {
+        const int i = 4 * (k * RULE_THREADS + threadIdx.x);
+        if (i >= n) continue;
+        const unsigned bits = words != nullptr ? words[i >> 5] >> (i & 31) : 0xfu;
+        const uint4 marks = reinterpret_cast<const uint4*>(mark)[i >> 2];
+        float e[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+        const unsigned mk[4] = {marks.x, marks.y, marks.z, marks.w};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            if (mk[c] != 0u) {
+                e[c] = e[c] > 0.0f ? e[c] / rep : e[c] * rep;
+                e[c] = e[c] - freq * (float)(mk[c] & 0x7fffffffu) - pres;
+            }
+            if (BIAS) {
+                const int b = bias_at[i + c];
+                if (b > 0) e[c] += p.bias_values[b - 1];
+            }
+            if (!((bits >> c) & 1u)) e[c] = -INFINITY;
+        }
+        if (p.vec && i + 4 <= n) {
+            *reinterpret_cast<float4*>(y + i) = make_float4(e[0], e[1], e[2], e[3]);
+        } else {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) if (i + c < n) y[i + c] = e[c];
+        }
+    }
+}
+
+PI_EXPORT int pi_logit_rules(const float* logits, long long ld, float* out, long long out_ld, int rows, int vocab, const int* history,
+                             const int* history_off, int history_total, const int* prompt_len, const float* repetition,
+                             const float* frequency, const float* presence, const int* bias_off, const int* bias_tokens,
+                             const float* bias_values, int bias_total, const void* mask, int mask_rows, const int* mask_row,
+                             cudaStream_t stream) {
+    if (rows <= 0) return 0;
+    if (vocab <= 0 || ld < vocab || out_ld < vocab) return pi_refuse("pi_logit_rules: vocab=%d ld=%lld out_ld=%lld", vocab, ld, out_ld);
+    if (rows > 65535) return pi_refuse("pi_logit_rules: %d rows are beyond the grid limit", rows);
+    if (vocab > 2147483647 - RULE_SLICE) return pi_refuse("pi_logit_rules: vocab=%d is beyond the limit", vocab);
+    RuleParams p;
+    p.logits = logits; p.ld = ld; p.out = out; p.out_ld = out_ld; p.vocab = vocab;
+    p.vec = (ld % 4 == 0 && out_ld % 4 == 0 && (((uintptr_t)logits | (uintptr_t)out) & 15) == 0) ? 1 : 0;
+    p.history = history; p.history_off = history_off; p.history_total = history_total; p.prompt_len = prompt_len;
+    p.repetition = repetition; p.frequency = frequency; p.presence = presence;
+    p.bias_off = bias_off; p.bias_tokens = bias_tokens; p.bias_values = bias_values; p.bias_total = bias_total;
+    p.mask = (const unsigned*)mask; p.mask_rows = mask_rows; p.mask_words = (vocab + 31) / 32; p.mask_row = mask_row;
+    const dim3 grid((vocab + RULE_SLICE - 1) / RULE_SLICE, rows), threads(RULE_THREADS);
+    if (bias_off != nullptr) pi_launch(logit_rules_kernel<true>, grid, threads, 0, stream, p);
+    else pi_launch(logit_rules_kernel<false>, grid, threads, 0, stream, p);
+    return pi_check_launch("pi_logit_rules");
 }

@@ -795,3 +795,61 @@ def logit_edit(logits: torch.Tensor, rows: torch.Tensor, tokens: torch.Tensor, v
     lib = _lib("sampling")
     _check(lib, lib.pi_logit_edit(_p(logits), c_int(logits.stride(0)), c_int(logits.shape[1]), _p(rows), _p(tokens),
                                   _p(values), c_int(n), c_int(1 if set_value else 0), _stream()), "logit_edit")
+
+
+_LOGIT_RULES = None      # (library, C function) once its argument types are declared
+
+
+def logit_rules(logits: torch.Tensor, history: torch.Tensor, history_off: torch.Tensor, prompt_len: torch.Tensor,
+                repetition: torch.Tensor, frequency: torch.Tensor, presence: torch.Tensor, bias_off: torch.Tensor | None = None,
+                bias_tokens: torch.Tensor | None = None, bias_values: torch.Tensor | None = None, mask: torch.Tensor | None = None,
+                mask_row: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """All rules of every row on float32 logits [n, V] in one pass.  Row r's token history is
+    ``history[history_off[r]:history_off[r + 1]]`` (int32), its first ``prompt_len[r]`` entries the prompt.  In this order:
+    a token of the history has its logit divided (if positive, else multiplied) by ``repetition[r]``; ``frequency[r]`` is
+    subtracted for each occurrence behind the prompt, ``presence[r]`` once if it occurs at all; ``bias_values`` of
+    ``bias_tokens[bias_off[r]:bias_off[r + 1]]`` are added (the last of several for one token counts); tokens whose bit is
+    zero in row ``mask_row[r]`` of ``mask`` (int32 [m, ceil(V / 32)], bit v % 32 of word v / 32; row -1, or one that is not
+    there: all allowed) become -inf.  ids outside the vocabulary are passed over.  ``out`` may be ``logits`` itself."""
+    global _LOGIT_RULES
+    tensors = (logits, history, history_off, prompt_len, repetition, frequency, presence, bias_off, bias_tokens, bias_values,
+               mask, mask_row, out)
+    _need_cuda(*tensors)
+    here = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != here:
+            raise KernelError(f"tensors must be on the current device cuda:{here}; got one on {t.device}")
+    if logits.dtype != torch.float32 or logits.dim() != 2 or logits.stride(1) != 1:
+        raise KernelError("logits must be float32 [rows, vocabulary] with unit stride")
+    n, V = logits.shape
+    for name, t, dtype, size in (("history", history, torch.int32, None), ("history_off", history_off, torch.int32, n + 1),
+                                 ("prompt_len", prompt_len, torch.int32, n), ("repetition", repetition, torch.float32, n),
+                                 ("frequency", frequency, torch.float32, n), ("presence", presence, torch.float32, n)):
+        if t.dtype != dtype or t.dim() != 1 or not t.is_contiguous() or (size is not None and t.numel() != size):
+            raise KernelError(f"logit_rules: '{name}' must be contiguous {dtype}{'' if size is None else f' of {size} values'}")
+    if (bias_off is None) != (bias_tokens is None) or (bias_off is None) != (bias_values is None) or (mask is None) != (mask_row is None):
+        raise KernelError("logit_rules: biases are offsets, tokens and values together, a mask goes with its rows")
+    if bias_off is not None and (bias_off.dtype != torch.int32 or bias_tokens.dtype != torch.int32 or bias_values.dtype != torch.float32
+                                 or tuple(bias_off.shape) != (n + 1,) or bias_tokens.shape != bias_values.shape
+                                 or not bias_off.is_contiguous() or not bias_tokens.is_contiguous() or not bias_values.is_contiguous()):
+        raise KernelError("logit_rules: bias_off int32 [rows + 1], bias_tokens int32 and bias_values float32 of one length")
+    if mask is not None and (mask.dtype != torch.int32 or mask.dim() != 2 or mask.shape[1] != (V + 31) // 32 or not mask.is_contiguous()
+                             or mask_row.dtype != torch.int32 or tuple(mask_row.shape) != (n,) or not mask_row.is_contiguous()):
+        raise KernelError(f"logit_rules: mask must be contiguous int32 [rows, {(V + 31) // 32}], mask_row int32 [{n}]")
+    if out is None:
+        out = torch.empty((n, V), dtype=torch.float32, device=logits.device)
+    elif out.dtype != torch.float32 or tuple(out.shape) != (n, V) or out.stride(1) != 1:
+        raise KernelError(f"logit_rules: out must be float32 [{n}, {V}] with unit stride")
+    if _LOGIT_RULES is None:
+        lib = _lib("sampling")
+        P, L = c_void_p, ctypes.c_longlong
+        lib.pi_logit_rules.argtypes = [P, L, P, L, c_int, c_int, P, P, c_int, P, P, P, P, P, P, P, c_int, P, c_int, P, P]
+        _LOGIT_RULES = (lib, lib.pi_logit_rules)
+    lib, fn = _LOGIT_RULES
+    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    _check(lib, fn(logits.data_ptr(), max(logits.stride(0), V), out.data_ptr(), max(out.stride(0), V), n, V, history.data_ptr(),
+                   history_off.data_ptr(), history.numel(), prompt_len.data_ptr(), repetition.data_ptr(), frequency.data_ptr(),
+                   presence.data_ptr(), ptr(bias_off), ptr(bias_tokens), ptr(bias_values),
+                   0 if bias_tokens is None else bias_tokens.numel(), ptr(mask), 0 if mask is None else mask.shape[0],
+                   ptr(mask_row), _stream()), "logit_rules")
+    return out

@@ -1,0 +1,26 @@
+"""The entry points around the 8-bit cache and the logit rules refuse tensors that are not on a CUDA device (no fallback)."""
+import pytest
+import torch
+
+
+def test_host_tensors_are_refused():
+    from pulse_infer_b200 import ops
+    i32 = lambda *shape: torch.zeros(shape, dtype=torch.int32)  # noqa: E731
+    bf = lambda *shape: torch.zeros(shape, dtype=torch.bfloat16)  # noqa: E731
+    pools = ops.cache_8bit_pools(2, 2, 16, 64, torch.int8, "cpu")
+    assert [tuple(t.shape) for t in pools] == [(2, 2, 16, 64), (2, 2, 1, 64, 16), (2, 2, 1), (2, 2, 1)]
+    calls = [lambda: ops.page_maps(i32(2, 3), i32(2), i32(2), i32(2), 16, 2),
+             lambda: ops.qk_norm_rope_write_8bit(bf(1, 512), None, None, 1e-6, None, None, True, *pools, torch.zeros(1, dtype=torch.int64), 4, 2, 64, i32(1)),
+             lambda: ops.pages_8bit_to_bf16(*pools, i32(1)),
+             lambda: ops.attention_decode_8bit(bf(1, 256), 256, *pools, i32(1, 1), i32(1), i32(1), i32(1), i32(1), 1, 1, 4, 2, 64, None, 0.1),
+             lambda: ops.logit_rules(torch.zeros(1, 10), i32(0), i32(2), i32(1), torch.ones(1), torch.zeros(1), torch.zeros(1))]
+    for call in calls:
+        with pytest.raises(ops.KernelError, match="CUDA device only"):
+            call()
+
+
+@pytest.mark.parametrize("bad", [(1, 2, 8, 64, torch.int8), (1, 2, 48, 64, torch.int8), (1, 2, 16, 96, torch.int8), (1, 2, 16, 64, torch.uint8)])
+def test_formats_that_do_not_exist(bad):
+    from pulse_infer_b200 import ops
+    with pytest.raises(ops.KernelError):
+        ops.cache_8bit_pools(*bad, "cpu")

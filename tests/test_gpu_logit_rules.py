@@ -1,0 +1,152 @@
+"""Penalties, biases and masks on logits against float64."""
+import numpy as np
+import pytest
+import torch
+
+from gpu_util import need_gpu
+
+pytestmark = pytest.mark.gpu
+
+
+def _ops():
+    from pulse_infer_b200 import ops
+    return ops
+
+
+def plain_rules(x, histories, prompts, rep, freq, pres, biases, masks):
+    """x [n, V] float64; per row: history, length of its prompt, penalties, [(token, value)], bool mask [V] or None.
+    Returns (result, bound on the error of 32-bit arithmetic): six roundings of numbers not above ``size``."""
+    x, size = x.copy(), np.abs(x)
+    for r in range(x.shape[0]):
+        for v in set(histories[r]):
+            if 0 <= v < x.shape[1]:
+                count = sum(1 for i, h in enumerate(histories[r]) if h == v and i >= prompts[r])
+                x[r, v] = x[r, v] / rep[r] if x[r, v] > 0 else x[r, v] * rep[r]
+                size[r, v] = max(size[r, v], abs(x[r, v])) + abs(freq[r] * count) + abs(pres[r])
+                x[r, v] -= freq[r] * count + pres[r]
+        last = {}
+        for v, b in biases[r]:
+            last[v] = b
+        for v, b in last.items():
+            if 0 <= v < x.shape[1]:
+                x[r, v] += b
+                size[r, v] += abs(b)
+        if masks[r] is not None:
+            x[r, ~masks[r]] = -np.inf
+    return x, 6 * 2.0 ** -24 * size
+
+
+def _case(rows, V, seed, history=200, with_bias=True, with_mask=True):
+    rng = np.random.RandomState(seed)
+    x = (3 * rng.randn(rows, V)).astype(np.float32)
+    lens = [0 if r == 1 else int(rng.randint(0, history + 1)) for r in range(rows)]
+    histories = [[int(v) for v in np.minimum(V * rng.rand(n) ** 3, V - 1)] for n in lens]
+    if rows > 2:
+        histories[2] += [0, V - 1, V - 1, -1, V, V + 7, 2 ** 31 - 1, -2 ** 31]          # the last ids, and some that are none
+    prompts = [int(rng.randint(0, len(h) + 1)) for h in histories]
+    f = lambda choices: rng.choice(choices, rows).astype(np.float32)  # noqa: E731
+    rep, freq, pres = f([1.0, 1.3, 0.8]), f([0.0, 0.7, -0.2]), f([0.0, 1.5])
+    biases = [[] for _ in range(rows)]
+    if with_bias:
+        biases = [[(int(v), float(np.float32(rng.randn()))) for v in rng.randint(0, V, rng.randint(0, 40))] for _ in range(rows)]
+        biases[0] += [(0, 1.0), (V - 1, -2.0), (0, 3.0), (-5, 1.0), (V, 1.0), (V - 1, -float("inf"))]
+    masks = [None if not with_mask or r % 3 == 0 else rng.rand(V) < 0.5 for r in range(rows)]
+    if with_mask and rows > 4:
+        masks[4] = np.zeros(V, dtype=bool)                                               # nothing is left
+    return x, histories, prompts, rep, freq, pres, biases, masks
+
+
+def _tensors(dev, V, histories, prompts, rep, freq, pres, biases, masks):
+    i32 = lambda v: torch.tensor(np.asarray(v, dtype=np.int64).astype(np.int32), device=dev)  # noqa: E731
+    f32 = lambda v: torch.tensor(np.asarray(v, dtype=np.float32), device=dev)  # noqa: E731
+    off = lambda rows: i32(np.concatenate([[0], np.cumsum([len(r) for r in rows])]))  # noqa: E731
+    flat = lambda rows: [v for r in rows for v in r]  # noqa: E731
+    args = [i32(flat(histories)), off(histories), i32(prompts), f32(rep), f32(freq), f32(pres)]
+    kw = {}
+    if any(biases):
+        kw.update(bias_off=off(biases), bias_tokens=i32([v for v, _ in flat(biases)]), bias_values=f32([b for _, b in flat(biases)]))
+    held = [m for m in masks if m is not None]
+    if held:
+        words = np.zeros((len(held), (V + 31) // 32 * 32), dtype=bool)
+        words[:, V:] = True
+        for i, m in enumerate(held):
+            words[i, :V] = m
+        words = np.packbits(words, axis=1, bitorder="little").view(np.uint32).view(np.int32)
+        at, rows = 0, []
+        for m in masks:
+            rows.append(-1 if m is None else at)
+            at += m is not None
+        kw.update(mask=torch.tensor(words.copy(), device=dev), mask_row=i32(rows))
+    return args, kw
+
+
+@pytest.mark.parametrize("rows,V", [(1, 151936), (5, 4096), (7, 4097), (3, 1), (6, 31), (9, 515), (5, 12291), (130, 2077)])
+@pytest.mark.parametrize("with_bias,with_mask", [(True, True), (False, False), (True, False), (False, True)])
+def test_logit_rules(rows, V, with_bias, with_mask):
+    dev, ops = need_gpu(), _ops()
+    x, *rules = _case(rows, V, rows + V, with_bias=with_bias, with_mask=with_mask)
+    want, bound = plain_rules(x.astype(np.float64), *rules)
+    args, kw = _tensors(dev, V, *rules)
+    src = torch.tensor(x, device=dev)
+    out = ops.logit_rules(src, *args, **kw)
+    assert torch.equal(src.cpu(), torch.tensor(x))
+    got = out.cpu().double().numpy()
+    fine = np.isfinite(want)
+    assert np.array_equal(fine, np.isfinite(got)) and np.array_equal(got[~fine], want[~fine])
+    assert (np.abs(got[fine] - want[fine]) <= bound[fine]).all()
+    # in place, and between rows that are further apart than the vocabulary
+    assert torch.equal(ops.logit_rules(src, *args, **kw, out=src), out) and torch.equal(src, out)
+    wide = torch.full((rows, V + 3), 5.0, device=dev)
+    wide[:, :V] = torch.tensor(x, device=dev)
+    apart = torch.full((rows, V + 7), 6.0, device=dev)
+    ops.logit_rules(wide[:, :V], *args, **kw, out=apart[:, :V])
+    assert torch.equal(apart[:, :V], out) and (apart[:, V:] == 6).all() and (wide[:, V:] == 5).all()
+
+
+def test_logit_rules_long_history_and_special_logits():
+    dev, ops = need_gpu(), _ops()
+    V, L = 5000, 70000
+    x, *rules = _case(2, V, 3, with_bias=False, with_mask=False)
+    rng = np.random.RandomState(0)
+    rules[0] = [[int(v) for v in rng.randint(0, 50, L)], [7] * 3]
+    rules[1] = [1000, 1]
+    x[0, 3], x[0, 4], x[1, 7] = -np.inf, np.inf, 0.0
+    want, bound = plain_rules(x.astype(np.float64), *rules)
+    args, kw = _tensors(dev, V, *rules)
+    got = ops.logit_rules(torch.tensor(x, device=dev), *args, **kw).cpu().double().numpy()
+    fine = np.isfinite(want)
+    assert np.array_equal(got[~fine], want[~fine]) and (np.abs(got[fine] - want[fine]) <= bound[fine]).all()
+
+
+def test_logit_rules_in_a_graph():
+    dev, ops = need_gpu(), _ops()
+    x, *rules = _case(4, 9000, 8)
+    args, kw = _tensors(dev, 9000, *rules)
+    src = torch.tensor(x, device=dev)
+    want = ops.logit_rules(src, *args, **kw)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = ops.logit_rules(src, *args, **kw)
+    got.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_what_logit_rules_refuses():
+    from pulse_infer_b200.ops import KernelError
+    dev, ops = need_gpu(), _ops()
+    i32 = lambda *shape: torch.zeros(shape, dtype=torch.int32, device=dev)  # noqa: E731
+    f32 = lambda *shape: torch.zeros(shape, device=dev)  # noqa: E731
+    base = dict(logits=f32(2, 70), history=i32(0), history_off=i32(3), prompt_len=i32(2), repetition=f32(2) + 1, frequency=f32(2), presence=f32(2))
+    ops.logit_rules(**base)
+    assert ops.logit_rules(**{**base, "logits": f32(0, 70), "history_off": i32(1), "prompt_len": i32(0), "repetition": f32(0), "frequency": f32(0),
+                              "presence": f32(0)}).shape == (0, 70)
+    for kw in (dict(logits=f32(2, 70).bfloat16()), dict(logits=f32(70, 2).T), dict(logits=f32(70)), dict(history=i32(1).long()), dict(history_off=i32(2)),
+               dict(prompt_len=i32(3)), dict(repetition=i32(2)), dict(frequency=f32(4)[::2]), dict(presence=f32(1)), dict(bias_off=i32(3)),
+               dict(bias_off=i32(3), bias_tokens=i32(2), bias_values=f32(1)), dict(bias_off=i32(2), bias_tokens=i32(1), bias_values=f32(1)),
+               dict(mask=i32(1, 3)), dict(mask=i32(1, 2), mask_row=i32(2)), dict(mask=i32(1, 3), mask_row=i32(1)), dict(mask=i32(3), mask_row=i32(2)),
+               dict(out=f32(2, 71)), dict(out=f32(2, 70).double()), dict(presence=torch.zeros(2))):
+        with pytest.raises(KernelError):
+            ops.logit_rules(**{**base, **kw})
