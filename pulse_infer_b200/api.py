@@ -21,7 +21,7 @@ class Engine:
                  max_tokens: int | None = None, max_batch_size: int = 8, chunk_size: int = 1024,
                  max_tokens_per_step: int | None = None, max_tokens_per_request: int | None = None,
                  use_cuda_graphs: bool = True, attention_impl: str = "auto", rope_pairing: str | None = None,
-                 lookahead: bool | None = None, kv_bytes: int | None = None):
+                 lookahead: bool | None = None, kv_bytes: int | None = None, cache_dtype: str | None = None):
         """``model``: folder with config.json and safetensors; or ``config`` + ``seed`` for random weights.
         The page pool is ``num_pages`` pages of ``page_size`` tokens, or what fits in ``kv_bytes`` bytes, or enough
         for ``max_tokens`` tokens
@@ -31,13 +31,16 @@ class Engine:
         one of 512 (the weights are read either way), and 1,024-token portions reach the prompt throughput of whole
         prompts, while a step stays short enough for the decoding requests that ride along.
         ``lookahead`` (default: on with CUDA graphs): a decode step stays in flight when ``step()`` returns and its
-        tokens are read while the next one runs; ``step()`` then returns the tokens of the step before."""
+        tokens are read while the next one runs; ``step()`` then returns the tokens of the step before.
+        ``cache_dtype`` 'float8_e4m3fn' or 'int8': keys and values are kept in 8 bits with a power-of-two scale for each
+        block of 16 tokens and kv head (dtype 'bfloat16', head sizes 64 and 128, page sizes 16 to 128): half the memory per
+        token, so twice the tokens in ``kv_bytes``, and half the bytes that decoding reads per key."""
         spec_options = {} if rope_pairing is None else {"rope_pairing": rope_pairing}
         self.runner = build_runner(model, config=config, seed=seed, dtype=dtype, device=device, page_size=page_size,
                                    num_pages=num_pages, max_tokens=max_tokens, max_requests=max(max_batch_size, 1),
                                    max_tokens_per_request=max_tokens_per_request,
                                    max_tokens_per_step=None, attention_impl=attention_impl,
-                                   use_cuda_graphs=use_cuda_graphs, kv_bytes=kv_bytes, **spec_options)
+                                   use_cuda_graphs=use_cuda_graphs, kv_bytes=kv_bytes, cache_dtype=cache_dtype, **spec_options)
         self.config = self.runner.config
         self.sampler = Sampler(self.runner.runtime.device)
         self.engine = ContinuousBatchEngine(self.runner, self.sampler, getattr(self.config, "eos_token_ids", ()),
@@ -48,9 +51,13 @@ class Engine:
     # ---- the reference engine's calls ------------------------------------------------------------------
     def add_request(self, prompt_tokens, max_new_tokens: int = 32, *, temperature: float = 0.0, top_k: int = 0,
                     top_p: float = 0.0, presence_penalty: float = 0.0, banned_tokens=(), seed: int = 0,
-                    ignore_eos: bool = False) -> int:
+                    ignore_eos: bool = False, repetition_penalty: float = 1.0, frequency_penalty: float = 0.0,
+                    logit_bias=(), grammar=None) -> int:
+        """``logit_bias``: {token: value} or (token, value) pairs.  For the other options see ``SamplingParams``."""
+        bias = tuple(logit_bias.items()) if hasattr(logit_bias, "items") else tuple(tuple(b) for b in logit_bias)
         params = SamplingParams(temperature=temperature, top_k=top_k, top_p=top_p, presence_penalty=presence_penalty,
-                                banned_tokens=tuple(banned_tokens), seed=seed)
+                                banned_tokens=tuple(banned_tokens), seed=seed, repetition_penalty=repetition_penalty,
+                                frequency_penalty=frequency_penalty, logit_bias=bias, grammar=grammar)
         return self.engine.add_request(list(prompt_tokens), max_new_tokens, params, ignore_eos)
 
     def step(self) -> list:

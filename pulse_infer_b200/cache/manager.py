@@ -41,11 +41,21 @@ class PageGroup:
     pool: torch.Tensor | None = None          # [caches, 2, pages, nkv, page_size, d]
     device_table: torch.Tensor | None = None  # int32 [slots, max_pages]
     first_live: dict = field(default_factory=dict)   # slot -> index of the first page still held
+    pools_8bit: list | None = None            # 8-bit pages: (keys, values, key scales, value scales) per cache
 
     def kv(self, cache_index: int):
-        """Key and value pools of one cache: two tensors [pages, nkv, page_size, d]."""
+        """Key and value pools of one cache: two tensors [pages, nkv, page_size, d] (8-bit pages: values transposed within
+        blocks of 16 tokens, [pages, nkv, page_size / 16, d, 16])."""
         local = self.cache_indices.index(cache_index)
+        if self.pools_8bit is not None:
+            return self.pools_8bit[local][:2]
         return self.pool[local, 0], self.pool[local, 1]
+
+    def scales(self, cache_index: int):
+        """Key and value scales of one cache, float32 [pages, nkv, page_size / 16]; (None, None) without 8-bit pages."""
+        if self.pools_8bit is None:
+            return None, None
+        return self.pools_8bit[self.cache_indices.index(cache_index)][2:]
 
 
 class CacheManager:
@@ -53,7 +63,8 @@ class CacheManager:
                  max_tokens_per_request: int, dtype: torch.dtype = torch.bfloat16, device=None,
                  allocate_pools: bool = True):
         """``cache_specs[i]`` is the CacheSpec of the model's cache i (or None); ``state_specs[j]`` is the
-        StateSpec of layer j (or None).  ``num_pages`` is the size of every group's pool."""
+        StateSpec of layer j (or None).  ``num_pages`` is the size of every group's pool.  ``dtype`` float8_e4m3fn or int8:
+        8-bit pages with a scale per 16 tokens and kv head (csrc/cache_8bit.cuh) instead of plain ones."""
         if page_size <= 0 or max_slots <= 0 or max_tokens_per_request <= 0:
             raise ValueError("page_size, max_slots and max_tokens_per_request must be positive")
         self.page_size = page_size
@@ -78,7 +89,11 @@ class CacheManager:
         for g in self.groups:
             g.device_table = torch.full((max_slots, self.max_pages_per_request), -1, dtype=torch.int32,
                                         device=self.device)
-            if allocate_pools:
+            if allocate_pools and dtype in (torch.float8_e4m3fn, torch.int8):
+                from ..ops.cache_8bit import cache_8bit_pools
+                g.pools_8bit = [cache_8bit_pools(num_pages, g.spec.num_kv_heads, page_size, g.spec.head_dim, dtype, self.device)
+                                for _ in g.cache_indices]
+            elif allocate_pools:
                 g.pool = torch.zeros((len(g.cache_indices), 2, num_pages, g.spec.num_kv_heads, page_size,
                                       g.spec.head_dim), dtype=dtype, device=self.device)
         # fixed-size per-request state, one tensor per layer that asks for it

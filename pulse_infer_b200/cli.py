@@ -52,6 +52,8 @@ def _common(ap: argparse.ArgumentParser) -> None:
     ap.add_argument("--page-size", type=int, default=16)
     ap.add_argument("--num-pages", type=int, default=None)
     ap.add_argument("--kv-gb", type=float, default=None, help="size the page pool by memory (GiB) instead of --num-pages")
+    ap.add_argument("--cache-dtype", choices=["auto", "float8_e4m3fn", "int8"], default="auto",
+                    help="keep keys and values in 8 bits with a scale per 16 tokens and kv head (bfloat16 only)")
     ap.add_argument("--max-tokens-per-step", type=int, default=None, help="token budget of one step (default: batch x chunk)")
     ap.add_argument("--print-logits-topk", type=int, default=0, metavar="K",
                     help="with every generated token, print the K largest logits it was chosen from")
@@ -76,7 +78,7 @@ def _make_engine(args, max_batch_size: int, chunk_size: int, num_pages: int | No
     kw = dict(dtype=args.dtype, device=args.device, page_size=args.page_size, num_pages=num_pages,
               max_tokens=None if kv_bytes else max_tokens, kv_bytes=kv_bytes,
               max_batch_size=max_batch_size, chunk_size=chunk_size, use_cuda_graphs=not args.no_cuda_graphs,
-              rope_pairing=pairing, max_tokens_per_step=args.max_tokens_per_step)
+              rope_pairing=pairing, max_tokens_per_step=args.max_tokens_per_step, cache_dtype=args.cache_dtype)
     if args.random_config:
         from .config.registry import architecture_name_of
         obj = read_json_file(args.random_config)
@@ -123,6 +125,8 @@ def qwen3_infer(argv=None) -> int:
     ap.add_argument("--top-k", type=int, default=None)
     ap.add_argument("--top-p", type=float, default=None)
     ap.add_argument("--presence-penalty", type=float, default=1.5)
+    ap.add_argument("--repetition-penalty", type=float, default=1.0)
+    ap.add_argument("--frequency-penalty", type=float, default=0.0)
     ap.add_argument("--greedy", action="store_true")
     args = ap.parse_args(argv)
     cfg = _config_first(args)
@@ -139,7 +143,8 @@ def qwen3_infer(argv=None) -> int:
     generated, t0 = 0, time.perf_counter()
     for i, prompt in enumerate(prompts):
         rid = engine.add_request(prompt, max_new, temperature=temperature, top_k=top_k, top_p=top_p,
-                                 presence_penalty=args.presence_penalty, seed=args.seed + i, ignore_eos=args.ignore_eos)
+                                 presence_penalty=args.presence_penalty, repetition_penalty=args.repetition_penalty,
+                                 frequency_penalty=args.frequency_penalty, seed=args.seed + i, ignore_eos=args.ignore_eos)
         engine.run_until_complete()
         out = engine.get_result(rid)
         generated += len(out)

@@ -10,7 +10,7 @@
 //                           position a + n - 1.  page_off is the exclusive prefix sum of their counts, page_list the pool
 //                           pages one behind the other, page_tokens the tokens [lo, hi) of each that can be seen, and
 //                           table[r, i] the place in page_list of the request's page i (-1: not listed).
-// Entries behind the last token or the last listed page are -1 (positions 0, page_tokens empty).
+// (A null table is left out.)  Entries behind the last token or the last listed page are -1 (positions 0, page_tokens empty).
 //
 // It is latency that counts: a decode step is a few hundred bytes.  So one launch does everything: every block scans the
 // R lengths for itself (a few kilobytes out of L2) and then fills its part of the outputs, looking its segment up in the
@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(PM_THREADS) page_maps_kernel(const PmParams p)
     __syncthreads();
 
     const int page_size = 1 << p.page_shift;
-    const long long cells = (long long)R * p.bt_stride;
+    const long long cells = p.table != nullptr ? (long long)R * p.bt_stride : 0;
     const long long total = (long long)p.num_tokens + p.num_listed + (R + 1) + cells;
     const long long begin = (long long)blockIdx.x * PM_PER_BLOCK;
     const long long end = min(begin + PM_PER_BLOCK, total);
@@ -156,7 +156,7 @@ PI_EXPORT int pi_page_maps(const int* block_table, int bt_rows, int bt_stride, c
     while ((1 << p.page_shift) < page_size) ++p.page_shift;
     p.slot_map = slot_map; p.positions = positions; p.token_seg = token_seg; p.seg_off = seg_off; p.page_off = page_off;
     p.page_list = page_list; p.page_tokens = (int2*)page_tokens; p.table = table; p.rows = rows;
-    const long long total = (long long)num_tokens + num_listed + num_segments + 1 + (long long)num_segments * bt_stride;
+    const long long total = (long long)num_tokens + num_listed + num_segments + 1 + (table != nullptr ? (long long)num_segments * bt_stride : 0);
     const long long blocks = (total + PM_PER_BLOCK - 1) / PM_PER_BLOCK;
     if (blocks > 2147483647LL) return pi_refuse("pi_page_maps: %lld entries are beyond the grid limit", total);
     const size_t smem = 2 * (size_t)(num_segments + 1) * sizeof(int);       // at most 32 KB: within the default limit

@@ -41,6 +41,9 @@ class CacheView:
     block_table: torch.Tensor | None   # int32 [slots, max_pages]
     page_size: int
     state: torch.Tensor | None = None  # [slots, *shape] fixed-size state of this layer, if it asked for one
+    # 8-bit pages: float32 [pages, nkv, page_size / 16]; values are then [pages, nkv, page_size / 16, d, 16]
+    key_scale: torch.Tensor | None = None
+    value_scale: torch.Tensor | None = None
 
 
 @dataclass
@@ -70,6 +73,7 @@ class StepContext:
         self.act_dtype = runtime.act_dtype
         self.device = runtime.device
         self.position_data: dict = {}
+        self.step_data: dict = {}        # what parts keep for one pass over the layers; emptied when a pass begins
         self.segments: list = []
         self._scratch: dict = {}
         self.splits_bound: int | None = None     # fixed number of key ranges (captured steps)
@@ -173,9 +177,32 @@ class StepContext:
             return CacheView(None, None, None, cm.page_size, state)
         group = cm.group_for_cache(cache_index)
         keys, values = group.kv(cache_index)
-        return CacheView(keys, values, group.device_table, cm.page_size, state)
+        return CacheView(keys, values, group.device_table, cm.page_size, state, *group.scales(cache_index))
 
-    def _decode_workspace(self, head_dim: int):
+    def page_maps(self, block_table: torch.Tensor, window: int | None) -> "ops.PageMaps":
+        """Slot map of the step, and the listed pages of its portions of prompts, for one group's block table: built once
+        per pass over the layers (not kept over passes: a recorded step has to build it again)."""
+        key = ("page_maps", block_table.data_ptr(), window)
+        maps = self.step_data.get(key)
+        if maps is None:
+            page = self.cache_manager.page_size
+            listed = sum((s.start + len(s.tokens) - 1) // page - (max(0, s.start - window + 1) // page if window else 0) + 1
+                         for s in self.segments if len(s.tokens) > 1) if self.has_prompt else 0
+            maps = self.step_data[key] = ops.page_maps(block_table, self.seg_slot, self.seg_start, self.seg_len, page,
+                                                       self.num_tokens, num_listed_pages=listed, window=window, min_tokens=2,
+                                                       with_table=self.has_prompt)
+        return maps
+
+    def expanded_pages(self, pages: int, num_kv_heads: int, head_dim: int) -> tuple:
+        """Room for that many 8-bit pages in bfloat16, keys and values: shared by the layers of a pass."""
+        shape = (pages, num_kv_heads, self.cache_manager.page_size, head_dim)
+        held = self.step_data.get(("expanded",) + shape)
+        if held is None:
+            held = tuple(torch.empty(shape, dtype=torch.bfloat16, device=self.device) for _ in range(2))
+            self.step_data[("expanded",) + shape] = held
+        return held
+
+    def decode_workspace(self, head_dim: int):
         """One workspace per head size for all layers and steps of a runtime: they run one after the other on one stream."""
         held = getattr(self.runtime, "decode_workspaces", None)
         if held is None:
@@ -199,7 +226,7 @@ class StepContext:
                 sc = AttentionScratch(1, None, None)
             elif ops.decode_on_tcgen05(head_dim, self.cache_manager.page_size, num_heads // max(num_kv_heads, 1), self.act_dtype,
                                        self.num_segments):
-                sc = AttentionScratch(1, None, None, decode_ws=self._decode_workspace(head_dim))
+                sc = AttentionScratch(1, None, None, decode_ws=self.decode_workspace(head_dim))
             else:
                 split_keys = (self.split_keys or {}).get((num_kv_heads, head_dim)) or ops.choose_split_keys(
                     len(self.decode_starts), num_kv_heads, self.decode_pos_max, head_dim)

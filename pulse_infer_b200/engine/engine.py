@@ -38,7 +38,8 @@ class ContinuousBatchEngine:
     def __init__(self, runner, sampler, eos_token_ids=(), max_batch_size: int = 8, chunk_size: int = 256,
                  max_tokens_per_step: int | None = None, max_sequences: int | None = None, lookahead: bool = False):
         """``runner``: the step function (``open``/``close`` happen through its cache manager);
-        ``sampler``: ``sample(logits, params, draw_index, history) -> token ids``.
+        ``sampler``: ``sample(logits, params, draw_index, history) -> token ids``; also with ``prompt_lens=`` when a
+        request's options tell its prompt from its output (``SamplingParams.needs_prompt_len``).
         ``lookahead`` needs ``sampler.sample_device`` and ``runner.step(..., tokens_from=)``."""
         self.runner = runner
         self.sampler = sampler
@@ -136,14 +137,16 @@ class ContinuousBatchEngine:
         if sampling_reqs:
             if self.logits_hook is not None:
                 self.logits_hook(sampling_reqs, logits)
-            history = None
-            if any(r.sampling.presence_penalty > 0.0 for r in sampling_reqs):
-                history = [r.all_tokens() if r.sampling.presence_penalty > 0.0 else () for r in sampling_reqs]
+            history, more = None, {}
+            if any(r.sampling.needs_history for r in sampling_reqs):
+                history = [r.token_array() if r.sampling.needs_history else () for r in sampling_reqs]
+                if any(r.sampling.needs_prompt_len for r in sampling_reqs):
+                    more = {"prompt_lens": [r.prompt_len() for r in sampling_reqs]}
             params = [r.sampling for r in sampling_reqs]
             draws = [r.num_generated() for r in sampling_reqs]
             rec.sampling_reqs = sampling_reqs
             if self.lookahead:
-                rec.tokens = self.sampler.sample_device(logits, params, draws, history)
+                rec.tokens = self.sampler.sample_device(logits, params, draws, history, **more)
                 self._start_read_back(rec)
                 # the next step may chain on this one if it is the steady state of decoding: one token each, all
                 # sampling, nothing that looks at earlier tokens on the host, and a step that takes device tokens
@@ -151,7 +154,7 @@ class ContinuousBatchEngine:
                                      and not any(p.edits_logits for p in params)
                                      and self.runner.takes_device_tokens(segments))
             else:
-                rec.tokens = self.sampler.sample(logits, params, draws, history)
+                rec.tokens = self.sampler.sample(logits, params, draws, history, **more)
             for r in sampling_reqs:
                 r.add_pending_token()
         return rec

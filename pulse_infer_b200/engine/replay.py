@@ -58,7 +58,8 @@ def replay_steps(runner, steps):
 
 
 def replay(model_dir: str, dtype: str, out_dir: str, max_tokens: int | None, lines, device="cuda:0", log=None,
-           page_size: int = PAGE_SIZE, num_pages: int | None = None, max_requests: int = MAX_LIVE_REQUESTS) -> int:
+           page_size: int = PAGE_SIZE, num_pages: int | None = None, max_requests: int = MAX_LIVE_REQUESTS,
+           cache_dtype: str | None = None) -> int:
     """Run the steps read from ``lines`` (an iterable of JSON strings); returns the number of steps.
     The pool holds ``num_pages`` pages of ``page_size`` tokens, or enough for ``max_tokens`` tokens (each request's
     count rounded up to a multiple of 64 or of the page size, whichever is larger).  Beside the ``.f32`` files,
@@ -74,7 +75,7 @@ def replay(model_dir: str, dtype: str, out_dir: str, max_tokens: int | None, lin
         num_pages = (pool_tokens + page_size - 1) // page_size
     pool_tokens = num_pages * page_size
     runner = build_runner(model_dir, dtype=dtype, device=device, page_size=page_size, num_pages=num_pages,
-                          max_requests=max_requests, max_tokens_per_request=pool_tokens)
+                          max_requests=max_requests, max_tokens_per_request=pool_tokens, cache_dtype=cache_dtype)
     out = log or sys.stdout
     count = 0
     index = []

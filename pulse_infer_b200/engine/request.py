@@ -13,6 +13,8 @@ import time
 from dataclasses import dataclass, field
 from enum import Enum
 
+import numpy as np
+
 from ..sampling.params import SamplingParams
 
 
@@ -38,6 +40,8 @@ class InferenceRequest:
     arrival_time: float = field(default_factory=time.monotonic)
     start_time: float | None = None
     finish_time: float | None = None
+    _array: object = field(default=None, repr=False)         # see token_array
+    _array_known: int = field(default=0, repr=False)
 
     # ---- inference_request.hpp:57-87 ------------------------------------------------------------------
     def prompt_len(self) -> int:
@@ -71,6 +75,23 @@ class InferenceRequest:
 
     def all_tokens(self) -> list:
         return self.prompt_tokens + self.generated_tokens
+
+    def token_array(self) -> np.ndarray:
+        """``all_tokens`` as an int32 array that grows with the request (penalties look at it every step); the caller does
+        not keep it."""
+        total, split = self.total_input_tokens(), len(self.prompt_tokens)
+        if self._array is None or self._array.size < total:
+            grown = np.empty(max(64, 2 * total), dtype=np.int32)
+            if self._array is None:
+                grown[:split] = self.prompt_tokens
+                self._array_known = split
+            else:
+                grown[:self._array_known] = self._array[:self._array_known]
+            self._array = grown
+        known = self._array_known
+        self._array[known:total] = self.generated_tokens[known - split:]
+        self._array_known = total - self.unresolved       # places of tokens still on the device are filled in again later
+        return self._array[:total]
 
     # ---- life cycle ----------------------------------------------------------------------------------------
     def start_running(self) -> None:

@@ -103,18 +103,19 @@ class PageMaps(NamedTuple):
     page_off: torch.Tensor       # int32 [R + 1] first listed page of a segment
     page_list: torch.Tensor      # int32 [N]     pool page of a listed page, -1: none
     page_tokens: torch.Tensor    # int32 [N, 2]  the tokens [first, end) of a listed page that the segment's queries can see
-    table: torch.Tensor          # int32 [R, W]  block table of the listed pages: places in page_list, -1: not listed
+    table: torch.Tensor | None   # int32 [R, W]  block table of the listed pages: places in page_list, -1: not listed
     rows: torch.Tensor           # int32 [R]     0 .. R - 1: segment r's row of ``table``
 
 
 def page_maps(block_table: torch.Tensor, seg_slot: torch.Tensor, seg_start: torch.Tensor, seg_len: torch.Tensor,
               page_size: int, num_tokens: int, num_listed_pages: int = 0, window: int | None = None,
-              min_tokens: int = 1) -> PageMaps:
+              min_tokens: int = 1, with_table: bool = True) -> PageMaps:
     """Block tables and slot maps of a step from the lengths of its requests, in one launch.  Segment r brings
     ``seg_len[r]`` tokens (0 is allowed) of the request in row ``seg_slot[r]`` of ``block_table`` (int32 [slots, W]), which
     holds ``seg_start[r]`` tokens already.  ``num_tokens`` and ``num_listed_pages`` size the outputs: the sums, or more
     (entries behind are -1), or less (what does not fit is left out).  Segments of at least ``min_tokens`` tokens list the
-    pages that their queries see, from the window's first on.  ``page_size``: a power of two."""
+    pages that their queries see, from the window's first on.  ``page_size``: a power of two.  ``with_table`` False: no
+    ``table`` (None), for a step that lists nothing."""
     _same_device(block_table, seg_slot, seg_start, seg_len)
     R = seg_slot.numel()
     _ints(torch.int32, (R,), seg_slot=seg_slot, seg_start=seg_start, seg_len=seg_len)
@@ -129,21 +130,22 @@ def page_maps(block_table: torch.Tensor, seg_slot: torch.Tensor, seg_start: torc
     slots, W = block_table.shape
     T, N = int(num_tokens), int(num_listed_pages)
     # one allocation for all of them, the 64-bit ones first
-    flat = torch.empty(4 * T + 3 * N + R * W + 3 * R + 2, dtype=torch.int32, device=block_table.device)
+    cells = R * W if with_table else 0
+    flat = torch.empty(4 * T + 3 * N + cells + 3 * R + 2, dtype=torch.int32, device=block_table.device)
     slot_map, positions, token_seg, page_tokens, seg_off, page_off, page_list, table, rows = flat.split(
-        [2 * T, T, T, 2 * N, R + 1, R + 1, N, R * W, R])
+        [2 * T, T, T, 2 * N, R + 1, R + 1, N, cells, R])
     if flat.numel() >= 2147483647:
         raise KernelError("page_maps: the maps are beyond 2^31 entries")
     base = flat.data_ptr()
     lib, fn = _bound("page_maps", "pi_page_maps", (_P, _I, _I, _P, _P, _P) + (_I,) * 6 + (_P,) * 10)
     at = [0, 2 * T, 3 * T, 4 * T, 4 * T + 2 * N, 4 * T + 2 * N + R + 1, 4 * T + 2 * N + 2 * R + 2,
-          4 * T + 3 * N + 2 * R + 2, 4 * T + 3 * N + 2 * R + 2 + R * W]
+          4 * T + 3 * N + 2 * R + 2, 4 * T + 3 * N + 2 * R + 2 + cells]
     ptr = [base + 4 * a for a in at]
     _k._check(lib, fn(block_table.data_ptr(), slots, W, seg_slot.data_ptr(), seg_start.data_ptr(), seg_len.data_ptr(), R,
-                      page_size, T, N, window or 0, min_tokens, ptr[0], ptr[1], ptr[2], ptr[4], ptr[5], ptr[6], ptr[3], ptr[7],
-                      ptr[8], _k._stream()), "page_maps")
+                      page_size, T, N, window or 0, min_tokens, ptr[0], ptr[1], ptr[2], ptr[4], ptr[5], ptr[6], ptr[3],
+                      ptr[7] if with_table else None, ptr[8], _k._stream()), "page_maps")
     return PageMaps(slot_map.view(torch.int64), positions, token_seg, seg_off, page_off, page_list, page_tokens.view(N, 2),
-                    table.view(R, W), rows)
+                    table.view(R, W) if with_table else None, rows)
 
 
 # ---- writing ----------------------------------------------------------------------------------------------------------
@@ -284,6 +286,8 @@ def attention_prompt_8bit(q: torch.Tensor, q_stride: int, kcache: torch.Tensor, 
     can share them.  Rows of single-token segments in ``out`` [num_tokens, nq d] are left as they are."""
     _same_device(q, kcache, vcache, seg_start, seg_len, out, maps.table)
     _, _, _, page_size, d = _check_pools(kcache, vcache, kscale, vscale, head_dim, nkv)
+    if maps.table is None:
+        raise KernelError("attention_prompt_8bit needs page maps with their table")
     out = _check_queries("attention_prompt_8bit", q, q_stride, num_tokens, nq, nkv, d, window, scale, out)
     R = maps.rows.numel()
     _ints(torch.int32, (R,), seg_start=seg_start, seg_len=seg_len)

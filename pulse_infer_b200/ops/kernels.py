@@ -89,7 +89,7 @@ def _need_contig(**tensors) -> None:
             raise KernelError(f"tensor '{name}' must be contiguous")
 
 
-def preload(head_dims=(), simple_attention: bool = False, float32_products: bool = False) -> None:
+def preload(head_dims=(), simple_attention: bool = False, float32_products: bool = False, cache_8bit: bool = False) -> None:
     """Build and load what a model needs, so that the first step does not pay for it.  Everything else
     (sampling, for instance) is built when it is first called."""
     _lib("elementwise")
@@ -100,6 +100,13 @@ def preload(head_dims=(), simple_attention: bool = False, float32_products: bool
         _lib("gemm_tcgen05")
     if simple_attention:
         _lib("attention_simple")
+    if cache_8bit:
+        for name in ("page_maps", "cache_8bit", "attention_8bit"):
+            _lib(name)
+        head_dims = [d for d in head_dims if d in (64, 128)]
+        for d in head_dims:
+            _lib("attention_tcgen05", d)
+        return
     for d in head_dims:
         _lib("attention_mma", d)
         if not float32_products and d in (64, 128) and os.environ.get("PULSE_TCGEN05_ATTENTION", "1") != "0":

@@ -7,7 +7,8 @@ queries and keys, keys (rotated) and values (raw) written to the pages of the to
 any query of the step attends, scores scaled by 1/sqrt(head size), causal by absolute position,
 kv head = head / (heads / kv heads), output projection without bias.
 The three projections are one product here (weights concatenated at load time); norm, rotation and the
-page write are one kernel.
+page write are one kernel.  With an 8-bit cache (``Runtime.cache_dtype``) that kernel encodes keys and values in blocks of
+16 tokens, decode attention reads the codes, and portions of prompts attend over the expanded pages of their requests.
 """
 from __future__ import annotations
 
@@ -42,6 +43,7 @@ class Attention(Mixer):
         self.o: torch.Tensor | None = None
         self.q_norm: torch.Tensor | None = None
         self.k_norm: torch.Tensor | None = None
+        self.cache_dtype = None             # set at load time: dtype of 8-bit pages
 
     @property
     def q_size(self) -> int:
@@ -56,7 +58,10 @@ class Attention(Mixer):
 
     def uses_key_ranges(self, page_size: int, act_dtype: torch.dtype) -> bool:
         """Whether decode steps of this layer cut each request's keys into ranges whose number must be bounded when a
-        step is recorded (the mma.sync decode kernel); the tcgen05 decode kernel divides the step's keys by itself."""
+        step is recorded (the mma.sync decode kernel); the tcgen05 decode kernel and the one for 8-bit pages divide the
+        step's keys by themselves."""
+        if self.cache_dtype is not None:
+            return False
         return not ops.decode_on_tcgen05(self.head_dim, page_size, self.num_heads // self.num_kv_heads, act_dtype)
 
     def tensor_specs(self) -> dict:
@@ -84,12 +89,14 @@ class Attention(Mixer):
             self.k_norm = tensors["k_norm.weight"].to(self.q_norm.dtype) if self.writes_cache else None
         self._tensors = {"qkv": self.qkv, "o": self.o}
         self.attention_impl = getattr(runtime, "attention_impl", "auto")
+        self.cache_dtype = getattr(runtime, "cache_dtype", None)
 
     def first_weights(self):
         return self.qkv
 
     takes_deferred_norm = True
     adds_to_residual = True
+    takes_8bit_cache = True
 
     def forward(self, x, ctx, cache, residual: torch.Tensor | None = None, next_norm=None):
         """x [T, H] in the activation dtype (or ``ops.NormedRows``: a norm that the first product finishes);
@@ -99,6 +106,9 @@ class Attention(Mixer):
         nkv_written = self.num_kv_heads if self.writes_cache else 0
         qkv = ops.linear(x, self.qkv, ctx.act_dtype)
         rot = ctx.position_data.get(self.position) if self.position else None
+        if cache.key_scale is not None:
+            attn = self._attend_8bit(qkv, rot, ctx, cache)
+            return ops.linear(attn, self.o, ctx.act_dtype, residual=residual, next_norm=next_norm)
         use_mma = (ctx.act_dtype == torch.bfloat16 and self.attention_impl != "simple"
                    and self.head_dim % 16 == 0 and self.head_dim <= 256)
         if use_mma and self.writes_cache and ctx.has_decode and not ctx.has_prompt and qkv.is_contiguous():
@@ -135,3 +145,28 @@ class Attention(Mixer):
                 ctx.num_tokens, self.num_heads, self.num_kv_heads, self.head_dim, cache.page_size, self.window,
                 self.scale)
         return ops.linear(attn, self.o, ctx.act_dtype, residual=residual, next_norm=next_norm)
+
+    def _attend_8bit(self, qkv, rot, ctx, cache):
+        """From the q/k/v product to the heads' outputs [T, nq d] over an 8-bit cache."""
+        nq, nkv, d = self.num_heads, self.num_kv_heads, self.head_dim
+        pools = (cache.keys, cache.values, cache.key_scale, cache.value_scale)
+        cos, sin, adjacent = (rot["cos"], rot["sin"], rot["adjacent"]) if rot else (None, None, True)
+        maps = ctx.page_maps(cache.block_table, self.window)
+        if self.writes_cache:
+            q = ops.qk_norm_rope_write_8bit(qkv, self.q_norm, self.k_norm, self.norm_eps, cos, sin, adjacent, *pools,
+                                            maps.slot_map, nq, nkv, d, ctx.error_count)
+        else:                                # the pages are another layer's: only the queries, in place
+            ops.qk_norm_rope_write(qkv, self.q_norm, None, self.norm_eps, cos, sin, adjacent, None, None, None, ctx.token_slot,
+                                   ctx.positions, cache.page_size, nq, 0, d, ctx.error_count)
+            q = qkv
+        out = torch.empty((ctx.num_tokens, nq * d), dtype=qkv.dtype, device=qkv.device)
+        if ctx.has_prompt:
+            keys, values = ctx.expanded_pages(maps.page_list.numel(), nkv, d)
+            ops.attention_prompt_8bit(q, nq * d, *pools, maps, ctx.seg_start, ctx.seg_len,
+                                      [(s.start, len(s.tokens)) for s in ctx.segments if len(s.tokens) > 1], ctx.num_tokens, nq, nkv,
+                                      d, self.window, self.scale, out=out, keys=keys, values=values)
+        if ctx.has_decode:
+            ops.attention_decode_8bit(q, nq * d, *pools, cache.block_table, ctx.seg_off, ctx.seg_slot, ctx.seg_start, ctx.seg_len,
+                                      ctx.num_tokens, ctx.num_segments, nq, nkv, d, self.window, self.scale,
+                                      workspace=ctx.decode_workspace(d), out=out)
+        return out

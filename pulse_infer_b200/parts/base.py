@@ -79,6 +79,9 @@ class Mixer(Part):
     #     float32 residual h itself; it then returns None, or the ``ops.NormedRows`` prepared for ``next_norm``
     takes_deferred_norm = False
     adds_to_residual = False
+    # forward() works with 8-bit pages: ``cache.key_scale`` / ``cache.value_scale`` are then given, and keys and values have
+    # the layout of csrc/cache_8bit.cuh
+    takes_8bit_cache = False
 
     def cache_spec(self) -> CacheSpec | None:
         return None

@@ -14,6 +14,10 @@ import torch
 from ..models.spec import ModelSpec
 from .base import ResidualStream, build_part
 
+# names of the 8-bit cache formats -> dtype of the pages (ops.CACHE_8BIT_DTYPES); None and "auto": the activation dtype
+CACHE_DTYPES = {None: None, "auto": None, "float8_e4m3fn": torch.float8_e4m3fn, "e4m3": torch.float8_e4m3fn,
+                "fp8": torch.float8_e4m3fn, "int8": torch.int8}
+
 
 @dataclass
 class Runtime:
@@ -22,6 +26,7 @@ class Runtime:
     device: torch.device
     mode: str = "bfloat16"
     attention_impl: str = "auto"     # 'auto' (tensor-core kernel in bfloat16) or 'simple'
+    cache_dtype: object = None       # None: pages in the activation dtype; 'float8_e4m3fn' / 'int8': 8-bit pages with scales
 
     def __post_init__(self):
         self.device = torch.device(self.device)
@@ -31,6 +36,15 @@ class Runtime:
             self.mode = "float32"
         if self.mode not in ("bfloat16", "float32"):
             raise ValueError(f"dtype must be 'bfloat16' or 'float32', got '{self.mode}'")
+        if not isinstance(self.cache_dtype, torch.dtype):
+            if self.cache_dtype not in CACHE_DTYPES:
+                raise ValueError(f"cache_dtype must be 'auto', 'float8_e4m3fn' or 'int8', got '{self.cache_dtype}'")
+            self.cache_dtype = CACHE_DTYPES[self.cache_dtype]
+        if self.cache_dtype is not None:
+            if self.cache_dtype not in (torch.float8_e4m3fn, torch.int8):
+                raise ValueError(f"cache_dtype must be float8_e4m3fn or int8, got {self.cache_dtype}")
+            if self.mode != "bfloat16" or self.attention_impl == "simple":
+                raise ValueError("an 8-bit cache goes with dtype 'bfloat16' and the tensor-core attention")
 
     @property
     def act_dtype(self) -> torch.dtype:
@@ -84,6 +98,20 @@ class DecoderModel:
 
     def cache_specs(self) -> list:
         return list(self._cache_specs)
+
+    def check_8bit_cache(self, page_size: int) -> None:
+        """Raise if some part cannot work with 8-bit pages of this size."""
+        from .. import ops
+        for entry in self.order:
+            mixer = self.layers[entry.layer].mixer
+            cs = mixer.cache_spec()
+            if cs is None:
+                continue
+            if not getattr(mixer, "takes_8bit_cache", False):
+                raise ValueError(f"layer {entry.layer}: a '{mixer.kind}' mixer does not work with an 8-bit cache")
+            if not ops.cache_8bit_usable(cs.head_dim, page_size):
+                raise ValueError(f"layer {entry.layer}: 8-bit pages take head sizes 64 and 128 and page sizes 16, 32, 64 and "
+                                 f"128, not head size {cs.head_dim} with page size {page_size}")
 
     def state_specs(self) -> list:
         return [layer.mixer.state_spec() for layer in self.layers]
@@ -148,6 +176,7 @@ class DecoderModel:
 
     # ---- one step -----------------------------------------------------------------------------------
     def forward(self, ctx) -> torch.Tensor:
+        ctx.step_data = {}
         ctx.position_data = {name: pe.prepare(ctx) for name, pe in self.positions.items()}
         hidden = self.embedding.forward(ctx.tokens, ctx)
         stream = ResidualStream(hidden, None)
@@ -158,6 +187,7 @@ class DecoderModel:
             cache = ctx.cache_view(entry.cache, entry.layer) if (entry.cache is not None or
                                                                 block.mixer.state_spec() is not None) else None
             block.forward(stream, ctx, cache)
+        ctx.step_data = {}
         if ctx.num_wanted == 0:
             return torch.empty((0, self.spec.vocab_size), dtype=torch.float32, device=hidden.device)
         x = self.final_norm.add_norm(stream.hidden, stream.pending, ctx, rows=ctx.want_rows,

@@ -1,7 +1,9 @@
 """Per-request sampling options, with the names and meanings the reference's generation demo uses
-(``demo/qwen3_infer.cpp:229-239,590-592``)."""
+(``demo/qwen3_infer.cpp:229-239,590-592``), and beside them the logit rules that the reference does not have: repetition and
+frequency penalty, biases, a grammar."""
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 
 
@@ -14,11 +16,37 @@ class SamplingParams:
     banned_tokens: tuple = ()       # never sampled (522-535)
     seed: int = 0                   # the draws of a request depend on (seed, index of the draw) only
     use_greedy: bool = False        # qwen3_infer.cpp:236
+    # in the order in which they apply (ops.logit_rules): repetition, frequency, presence, biases and bans, grammar
+    repetition_penalty: float = 1.0  # logits of tokens in prompt or output are divided by it if positive, else multiplied
+    frequency_penalty: float = 0.0   # subtracted once for every time a token was generated
+    logit_bias: tuple = ()           # (token, value) pairs that are added
+    # an object with ``token_mask(generated) -> None or ceil(vocabulary / 32) 32-bit words`` (bit v % 32 of word v / 32 set:
+    # token v is allowed), asked before every token with the tokens generated so far
+    grammar: object = None
+
+    def __post_init__(self):
+        if not (self.repetition_penalty > 0.0 and math.isfinite(self.repetition_penalty)):
+            raise ValueError(f"repetition_penalty must be positive and finite, got {self.repetition_penalty}")
+        if not math.isfinite(self.frequency_penalty):
+            raise ValueError(f"frequency_penalty must be finite, got {self.frequency_penalty}")
+        if self.grammar is not None and not callable(getattr(self.grammar, "token_mask", None)):
+            raise ValueError("a grammar needs a token_mask(generated) method")
 
     @property
     def greedy(self) -> bool:
         return self.use_greedy or self.temperature <= 0.0
 
     @property
+    def needs_history(self) -> bool:
+        """Whether the tokens so far have a say in the next one."""
+        return (self.presence_penalty > 0.0 or self.repetition_penalty != 1.0 or self.frequency_penalty != 0.0
+                or self.grammar is not None)
+
+    @property
+    def needs_prompt_len(self) -> bool:
+        """Whether it matters which of the tokens so far were generated."""
+        return self.frequency_penalty != 0.0 or self.grammar is not None
+
+    @property
     def edits_logits(self) -> bool:
-        return self.presence_penalty > 0.0 or bool(self.banned_tokens)
+        return self.needs_history or bool(self.banned_tokens) or bool(self.logit_bias)

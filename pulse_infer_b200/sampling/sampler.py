@@ -3,13 +3,15 @@
 Greedy rows use the argmax kernel; rows with a temperature use the sampling kernel (temperature,
 top-k, top-p; a counter-based uniform draw keyed by the request's seed and the index of the draw, so
 a request's tokens do not depend on what else is in the batch or on being recomputed after a
-preemption).  Presence penalty and banned ids edit single logits first.
+preemption).  Penalties, biases, banned ids and grammars are applied to the logits first, all of a step's in one
+kernel (``ops.logit_rules``) whose inputs travel in one copy.
 
 Reference parity: ``src/scheduler/continuous_batch_engine.cpp:237,259-305`` (greedy on the last row of
 each request) and ``demo/qwen3_infer.cpp:229-423`` (the sampler of the single-stream demo).
 """
 from __future__ import annotations
 
+import numpy as np
 import torch
 
 from .. import ops
@@ -69,33 +71,68 @@ class Sampler:
         self._copied[i].record()
         return dev
 
-    def sample(self, logits: torch.Tensor, params: list, draw_index: list, history: list | None = None) -> list:
+    def sample(self, logits: torch.Tensor, params: list, draw_index: list, history: list | None = None,
+               prompt_lens: list | None = None) -> list:
         """logits float32 [n, V]; params[i] SamplingParams; draw_index[i] how many tokens request i has
-        drawn so far; history[i] the tokens a presence penalty looks at.  Returns n token ids."""
-        out = self.sample_device(logits, params, draw_index, history)
+        drawn so far; history[i] the tokens that penalties and grammars look at (ids, a list or an int32 array), its first
+        prompt_lens[i] (default: none) the prompt.  Returns n token ids."""
+        out = self.sample_device(logits, params, draw_index, history, prompt_lens)
         return [] if out is None else out.tolist()
 
-    def sample_device(self, logits: torch.Tensor, params: list, draw_index: list, history: list | None = None):
+    def _apply_rules(self, logits: torch.Tensor, params: list, history: list | None, prompt_lens: list | None) -> torch.Tensor:
+        """``logits`` after the rules of every row, in a new tensor."""
+        n, V = logits.shape
+        told = history is not None
+        tokens = [np.asarray(history[i], dtype=np.int32) if told and p.needs_history else np.empty(0, np.int32)
+                  for i, p in enumerate(params)]
+        prompts = [min(int(prompt_lens[i]), tokens[i].size) if prompt_lens is not None else 0 for i in range(n)]
+        biases = []
+        for p in params:
+            row = {int(t): float(v) for t, v in p.logit_bias}
+            row.update((int(t), float("-inf")) for t in p.banned_tokens)
+            biases.append(row)
+        words = (V + 31) // 32
+        masks, mask_row = [], [-1] * n
+        for i, p in enumerate(params):
+            mask = p.grammar.token_mask(tokens[i][prompts[i]:].tolist()) if p.grammar is not None else None
+            if mask is not None:
+                mask = np.ascontiguousarray(mask).reshape(-1)
+                if mask.size != words or mask.dtype.itemsize != 4 or mask.dtype.kind not in "iu":
+                    raise ValueError(f"a token mask must hold {words} 32-bit words, got {mask.size} of {mask.dtype}")
+                mask_row[i] = len(masks)
+                masks.append(mask.view(np.int32))
+        f32 = lambda v: np.asarray(v, dtype=np.float32).view(np.int32)  # noqa: E731
+        off = lambda v: np.concatenate([[0], np.cumsum(v)]).astype(np.int32)  # noqa: E731
+        with_history = [p.needs_history and told for p in params]
+        parts = [off([t.size for t in tokens]), np.asarray(prompts, np.int32),
+                 f32([p.repetition_penalty if h else 1.0 for p, h in zip(params, with_history)]),
+                 f32([p.frequency_penalty if h else 0.0 for p, h in zip(params, with_history)]),
+                 f32([p.presence_penalty if h and p.presence_penalty > 0.0 else 0.0 for p, h in zip(params, with_history)]),
+                 np.concatenate(tokens), off([len(b) for b in biases]), np.asarray([t for b in biases for t in b], np.int32),
+                 f32([v for b in biases for v in b.values()]), np.asarray(mask_row, np.int32),
+                 np.concatenate(masks) if masks else np.empty(0, np.int32)]
+        host = torch.from_numpy(np.concatenate(parts))
+        if self.device.type == "cuda":
+            host = host.pin_memory()
+        (history_off, prompt_len, repetition, frequency, presence, flat, bias_off, bias_tokens, bias_values, rows,
+         mask) = host.to(self.device, non_blocking=True).split([p.size for p in parts])
+        as_f32 = lambda t: t.view(torch.float32)  # noqa: E731
+        kw = {}
+        if bias_tokens.numel():
+            kw.update(bias_off=bias_off, bias_tokens=bias_tokens, bias_values=as_f32(bias_values))
+        if masks:
+            kw.update(mask=mask.view(len(masks), words), mask_row=rows)
+        return ops.logit_rules(logits, flat, history_off, prompt_len, as_f32(repetition), as_f32(frequency), as_f32(presence), **kw)
+
+    def sample_device(self, logits: torch.Tensor, params: list, draw_index: list, history: list | None = None,
+                      prompt_lens: list | None = None):
         """The same, but the token ids stay on the device (int32 [n], or None for no rows): the caller reads them
         when it needs them, and the next step can take them as its input without a round trip."""
         n = logits.shape[0]
         if n == 0:
             return None
         if any(p.edits_logits for p in params):
-            logits = logits.clone()
-            rows, toks, vals_add, rows_set, toks_set = [], [], [], [], []
-            for i, p in enumerate(params):
-                if p.presence_penalty > 0.0 and history is not None:
-                    for t in set(history[i]):
-                        rows.append(i); toks.append(t); vals_add.append(-p.presence_penalty)
-                for t in set(p.banned_tokens):
-                    rows_set.append(i); toks_set.append(t)
-            mk = lambda v, dt: torch.tensor(v, dtype=dt, device=self.device)  # noqa: E731
-            if rows:
-                ops.logit_edit(logits, mk(rows, torch.int32), mk(toks, torch.int32), mk(vals_add, torch.float32), False)
-            if rows_set:
-                ops.logit_edit(logits, mk(rows_set, torch.int32), mk(toks_set, torch.int32),
-                               mk([float("-inf")] * len(rows_set), torch.float32), True)
+            logits = self._apply_rules(logits, params, history, prompt_lens)
         if all(p.greedy for p in params):
             return ops.argmax(logits)
         self._ensure_tables()

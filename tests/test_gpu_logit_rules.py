@@ -150,3 +150,71 @@ def test_what_logit_rules_refuses():
                dict(out=f32(2, 71)), dict(out=f32(2, 70).double()), dict(presence=torch.zeros(2))):
         with pytest.raises(KernelError):
             ops.logit_rules(**{**base, **kw})
+
+
+class _Grammar:
+    """Allows, after k generated tokens, the ids that are k modulo 7; everything after the fourth."""
+
+    def __init__(self, vocab):
+        self.vocab, self.seen = vocab, []
+
+    def token_mask(self, generated):
+        self.seen.append(list(generated))
+        if len(generated) >= 4:
+            return None
+        bits = np.zeros((self.vocab + 31) // 32 * 32, dtype=bool)
+        bits[len(generated):self.vocab:7] = True
+        return np.packbits(bits, bitorder="little").view(np.uint32)
+
+
+def test_sampler_applies_the_rules_of_every_request():
+    from pulse_infer_b200.sampling import Sampler, SamplingParams
+    dev = need_gpu()
+    V = 2077
+    x = (3 * np.random.RandomState(4).randn(7, V)).astype(np.float32)
+    grammar = _Grammar(V)
+    params = [SamplingParams(), SamplingParams(presence_penalty=1.5), SamplingParams(repetition_penalty=1.3, frequency_penalty=0.7),
+              SamplingParams(banned_tokens=(3, 5, 3), logit_bias=((9, 4.0), (3, 2.0))), SamplingParams(grammar=grammar),
+              SamplingParams(presence_penalty=0.3, repetition_penalty=0.9, frequency_penalty=0.2, logit_bias=((1, -1.0),), banned_tokens=(0,)),
+              SamplingParams(temperature=0.7, top_k=5, presence_penalty=2.0, seed=3)]
+    histories = [[], [1, 2, 2, 3], [4, 4, 5, 6, 6], [3, 9], [8, 8, 2], list(range(50)) * 2, [int(np.argmax(x[6]))]]
+    prompts = [0, 4, 2, 0, 1, 50, 0]
+    rep = [p.repetition_penalty for p in params]
+    freq = [p.frequency_penalty for p in params]
+    pres = [p.presence_penalty for p in params]
+    biases = [list(p.logit_bias) + [(t, -np.inf) for t in p.banned_tokens] for p in params]
+    masks = [None] * 7
+    masks[4] = np.arange(V) % 7 == 2
+    used = [h if p.needs_history else [] for h, p in zip(histories, params)]
+    want, _ = plain_rules(x.astype(np.float64), used, prompts, rep, freq, pres, biases, masks)
+    src = torch.tensor(x, device=dev)
+    sampler = Sampler(dev)
+    got = sampler.sample(src, params, [0] * 7, histories, prompts)
+    assert got[:6] == [int(np.argmax(w)) for w in want[:6]] and torch.equal(src.cpu(), torch.tensor(x))
+    assert got[6] in np.argsort(-want[6])[:5] and grammar.seen == [[8, 2]]
+    # as before: no history, no penalty; presence alone without the lengths of the prompts
+    assert sampler.sample(src[1:2], [params[1]], [0]) == [int(np.argmax(x[1]))]
+    assert sampler.sample(src[1:2], [params[1]], [0], [histories[1]]) == [int(np.argmax(want[1]))]
+    bad = _Grammar(V)
+    bad.token_mask = lambda generated: np.zeros(3, dtype=np.int32)
+    with pytest.raises(ValueError, match="token mask"):
+        sampler.sample(src[:1], [SamplingParams(grammar=bad)], [0], [[]], [0])
+
+
+def test_engine_generates_under_rules(model_folders):
+    """Through Engine: a grammar sees what was generated, a repeated token is penalised out, biases choose."""
+    from pulse_infer_b200 import Engine
+    from tiny_configs import CONFIGS
+    need_gpu()
+    V = CONFIGS["A"].vocab_size
+    engine = Engine(model_folders["A"], dtype="float32", page_size=8, num_pages=40, max_batch_size=4)
+    grammar = _Grammar(V)
+    a = engine.add_request([1, 2, 3], 6, ignore_eos=True, grammar=grammar)
+    b = engine.add_request([4, 5], 12, ignore_eos=True, frequency_penalty=1e4)
+    c = engine.add_request([4, 5], 5, ignore_eos=True, logit_bias={17: 1e4})
+    d = engine.add_request([4, 5], 12, ignore_eos=True, repetition_penalty=1e6)
+    engine.run_until_complete()
+    out = [engine.get_result(i) for i in (a, b, c, d)]
+    assert [t % 7 for t in out[0][:4]] == [0, 1, 2, 3] and grammar.seen == [out[0][:i] for i in range(6)]
+    assert len(set(out[1])) == 12 and out[2] == [17] * 5
+    assert len(out[3]) == 12

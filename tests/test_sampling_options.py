@@ -1,0 +1,44 @@
+"""Sampling options on the host: what they ask for, what they refuse, and the token array of a request."""
+import numpy as np
+import pytest
+
+from pulse_infer_b200.engine.request import InferenceRequest
+from pulse_infer_b200.sampling import SamplingParams
+
+
+def test_what_the_options_look_at():
+    assert not SamplingParams().edits_logits and not SamplingParams().needs_history
+    for kw in (dict(repetition_penalty=1.1), dict(frequency_penalty=-0.5), dict(presence_penalty=1.0)):
+        p = SamplingParams(**kw)
+        assert p.edits_logits and p.needs_history
+    assert SamplingParams(frequency_penalty=0.1).needs_prompt_len and not SamplingParams(presence_penalty=0.1).needs_prompt_len
+    for kw in (dict(logit_bias=((3, 1.0),)), dict(banned_tokens=(4,))):
+        p = SamplingParams(**kw)
+        assert p.edits_logits and not p.needs_history
+    assert not SamplingParams(presence_penalty=-1.0).needs_history
+
+
+@pytest.mark.parametrize("kw", [dict(repetition_penalty=0.0), dict(repetition_penalty=-1.0), dict(repetition_penalty=float("nan")),
+                                dict(repetition_penalty=float("inf")), dict(frequency_penalty=float("nan")), dict(grammar=object())])
+def test_options_that_are_refused(kw):
+    with pytest.raises(ValueError):
+        SamplingParams(**kw)
+
+
+def test_token_array_follows_the_request():
+    req = InferenceRequest(0, [5, 6, 7], 500)
+    assert req.token_array().tolist() == [5, 6, 7]
+    for t in range(100):
+        req.add_sampled_token(t, ())
+        assert req.token_array().tolist() == req.all_tokens()
+    req.add_pending_token()
+    assert req.token_array().tolist() == req.all_tokens()
+    req.add_pending_token()
+    req.token_array()
+    req.resolve_pending_token(77, ())
+    assert req.token_array().tolist() == req.all_tokens() and req.token_array()[-2] == 77
+    req.drop_pending_tokens()
+    assert req.token_array().tolist() == req.all_tokens()
+    req.preempt()
+    req.add_sampled_token(9, ())
+    assert req.token_array().tolist() == req.all_tokens() and req.token_array().dtype == np.int32
