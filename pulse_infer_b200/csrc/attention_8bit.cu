@@ -1,9 +1,11 @@
 // Decode attention over 8-bit key/value pages (format: cache_8bit.cuh): segments of one token,
 //   out = softmax(scale * q K^T) V,  K = 2^ek k8,  V = 2^ev v8,  keys lo .. pos (lo = pos - window + 1 with a window)
 //
-// All of it is memory traffic - each byte of a key or value is used for a handful of query heads - so the keys and values
-// go straight from memory into the registers in which mma.sync wants them, in 16-byte pieces, and nothing is exchanged
-// between the warps of a CTA until a piece of work ends.  A warp takes 64 keys (four blocks of 16) at a time:
+// All of it is memory traffic - each byte of a key or value is used for a handful of query heads.  A warp takes 64 keys (four
+// blocks of 16) at a time, in four units (two of keys, two of values, 4 KB each for D = 128), which come through a queue in
+// shared memory that belongs to it alone: bulk copies of half a block, an mbarrier per unit, no exchange between warps, and
+// 128 to 160 KB per SM in flight.  (Lanes that fetch their 16-byte operand pieces themselves, into registers or with
+// cp.async, ask for 32 or 64 bytes of a line at a time; that path delivers 4.7 and 4.0 TB/s, from L2 no more.)
 //   S^T = K Q^T      m16n8k16, 16 keys x 8 query heads; the codes become half precision exactly (two instructions for four
 //                    e4m3, five for int8), queries are scaled to [1, 2) per head so that half precision holds them
 //   softmax          in 32 bits; a value block's scale joins the exponent: w = 2^(s + ev - m'), m' the running maximum of
@@ -16,21 +18,32 @@
 //   elements lane t of a quad holds elements 64 c + 16 t .. + 15 of its rows, four of them per k step
 //   tokens   lane t of a quad holds block t of each line of V^T, four tokens per k step j: those of the keys' tile j
 //
-// Work split: as in the tcgen05 decode kernel.  The 64-key tiles of all (request, kv head, eight query heads) triples form
-// one sequence, `pair_cost` units before each, and every CTA (one per SM) takes an equal span of it.  A triple inside one
-// span is finished by its CTA; a cut one leaves (maximum, sum, accumulator) per piece in the workspace, and the CTA that
-// delivers its last missing piece adds the pieces up in the order of the keys.  Nothing waits for another CTA.  Within a
-// piece the eight warps take tiles in turn and are added up in warp order through shared memory.
+// Work split: the 64-key tiles of all (request, kv head, eight query heads) triples form one sequence, `pair_cost` units
+// before each; every CTA (one per SM) takes an equal share of it and every warp an equal share of its CTA's, whatever the
+// lengths of the requests.  A warp runs through its pieces without waiting for another warp, asking ahead across the
+// boundaries of pieces.  A triple inside one warp's share is written by that warp.  The others are added up through shared
+// memory, once, when all warps are done; what was cut between CTAs leaves (maximum, sum, accumulator) in the workspace, and the
+// CTA that delivers a triple's last missing piece adds the pieces up in the order of the keys.  Nothing waits for another CTA.
 // A group of more than eight query heads is cut in pieces of eight, and its keys are read once for each (from L2 mostly).
+//
+// Measured (B200, e4m3, 8 kv heads of 128; device time of a launch among others): 64 requests of 130 to 8,190 keys, 40 query
+// heads: 83 us, 459 MB at 5.5 TB/s (6.9 while the queues run); 8 requests of 4,096 keys: 22 us, of which 10 are transfer, 4
+// the way to the first byte (lengths, block table, copies: three round trips) and 6 the sums between warps and CTAs at the end.
+// Every wait is bounded; after one that ran out the kernel records a code and goes on without data.
 #include <math.h>
 
 #include "cache_8bit.cuh"
 
+// 8 warps with 5 units each (12 with 3: the same within 3 %, 10 with 4 no better)
 #define A8_WARPS 8
+#define A8_RING 5              // units of a warp's queue for D = 128, twice as many for D = 64
 #define A8_THREADS (A8_WARPS * 32)
 #define A8_TILE 64
 #define A8_HEADS 8
 #define A8_MAX_SEGS 1024
+#ifndef A8_SPIN_LIMIT
+#define A8_SPIN_LIMIT (1u << 22)
+#endif
 #define A8_SLOT_HEADS 16       // heads per slot of the workspace
 
 struct A8Params {
@@ -47,12 +60,30 @@ struct A8Params {
     float scale_log2;
 };
 
-struct A8Piece {
-    int seg, kvh, h0, heads, pos, lo, tile, ntiles;   // tile: first 64-key tile of the piece (absolute)
-    int whole, slot, cta_first, pieces;
+// what the kernel needs of the segments, in shared memory
+struct A8Meta {
+    int pre[A8_MAX_SEGS + 1];       // first unit of a segment; pre[num_segments]: their number
+    int pos[A8_MAX_SEGS], slot[A8_MAX_SEGS], row[A8_MAX_SEGS];
 };
 
-struct A8Cursor { int f, end, seg, span; };
+struct A8Piece {
+    int seg, slot, kvh, h0, heads, pos, lo, tile, ntiles;   // tile: first 64-key tile of the piece (absolute)
+    int unit0, tiles;                                  // unit of the triple's first tile, and how many tiles the triple has
+    int begins, ends;                                  // the piece holds the triple's first / last tile
+};
+
+struct A8Cursor { int f, end, seg; };
+
+// n units in equal shares
+struct A8Shares {
+    int each, more;                 // the first `more` shares have each + 1 units
+    __device__ __forceinline__ A8Shares(int n, int shares) : each(n / shares), more(n - n / shares * shares) {}
+    __device__ __forceinline__ int from(int share) const { return share * each + min(share, more); }
+    __device__ __forceinline__ int holds(int unit) const {      // the share of a unit
+        const int longer = more * (each + 1);
+        return unit < longer ? unit / (each + 1) : more + (unit - longer) / each;
+    }
+};
 
 __device__ __forceinline__ float a8_ex2(float x) {
     float y;
@@ -71,151 +102,278 @@ __device__ __forceinline__ unsigned a8_turn(unsigned x) {
     return y;
 }
 
-__device__ __forceinline__ uint4 a8_load(const unsigned char* p) {
-    uint4 v;
-    // not the read-only path: the pages were written by the kernel before this one, which may still have been running when
-    // this kernel began
-    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
+__device__ __forceinline__ void a8_copy4(unsigned dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void a8_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void a8_wait_group() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void a8_bulk(unsigned dst, const void* src, unsigned bytes, unsigned bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+                 "r"(bytes), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void a8_expect(unsigned bar, unsigned bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+// false: the wait ran out (A8_SPIN_LIMIT polls); the status word then names the warp and the unit
+__device__ unsigned g_a8_status;
+__device__ __forceinline__ bool a8_arrived(unsigned bar, unsigned parity, unsigned code) {
+    for (unsigned i = 0; i < A8_SPIN_LIMIT; ++i) {
+        unsigned done;
+        asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+                     : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+        if (done) return true;
+    }
+    atomicCAS(&g_a8_status, 0u, code);
+    return false;
 }
 
 __device__ __forceinline__ unsigned a8_word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
-// the newest position of a segment, kept within the block table
-__device__ __forceinline__ int a8_pos(const A8Params& p, int seg) {
-    const long long most = ((long long)p.bt_stride << p.page_shift) - 1;
-    return (int)min((long long)p.seg_start[seg], most);
-}
 __device__ __forceinline__ int a8_lo(const A8Params& p, int pos) { return p.window > 0 ? max(0, pos - p.window + 1) : 0; }
-__device__ __forceinline__ int a8_seg_tiles(const A8Params& p, int seg) {
-    if (p.seg_len[seg] != 1) return 0;
-    const int pos = a8_pos(p, seg);
-    return pos < 0 ? 0 : pos / A8_TILE - a8_lo(p, pos) / A8_TILE + 1;
-}
-// pre[s]: tiles per triple of the segments before s, pre[A8_MAX_SEGS + 1 + s]: decoding segments before s
-__device__ __forceinline__ int a8_seg_unit(const A8Params& p, const int* pre, int s) {
-    return p.nkv * p.head_tiles * (pre[s] + p.pair_cost * pre[A8_MAX_SEGS + 1 + s]);
-}
 
-__device__ __forceinline__ void a8_begin(const A8Params& p, const int* pre, A8Cursor& c) {
-    const int total = a8_seg_unit(p, pre, p.num_segments);
-    c.span = max((total + (int)gridDim.x - 1) / (int)gridDim.x, p.span_min);
-    const long long b = (long long)blockIdx.x * c.span;
-    c.f = (int)(b < total ? b : total);
-    c.end = (int)min((long long)c.f + c.span, (long long)total);
+// a cursor over the units [from, to) of the sequence
+__device__ __forceinline__ void a8_begin(const A8Params& p, const A8Meta& meta, int from, int to, A8Cursor& c) {
+    c.f = from;
+    c.end = to;
     int lo = 0, hi = p.num_segments;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (a8_seg_unit(p, pre, mid) <= c.f) lo = mid; else hi = mid;
+        if (meta.pre[mid] <= from) lo = mid; else hi = mid;
     }
     c.seg = lo;
 }
 
-__device__ __forceinline__ bool a8_next(const A8Params& p, const int* pre, A8Cursor& c, A8Piece& w) {
-    while (c.f < c.end) {
-        while (a8_seg_unit(p, pre, c.seg + 1) <= c.f) ++c.seg;       // ends: f lies before the end of the sequence
-        const int n = pre[c.seg + 1] - pre[c.seg];
-        const int per = n + p.pair_cost;
-        const int rel = c.f - a8_seg_unit(p, pre, c.seg);
-        const int tile0 = c.f - rel % per + p.pair_cost;              // unit of the triple's first tile
-        const int lo_u = max(c.f, tile0), hi_u = min(c.end, tile0 + n);
-        if (hi_u <= lo_u) { c.f = c.end; break; }                     // the span ends among the cost units
-        const int triple = rel / per, ht = triple % p.head_tiles;
-        w.seg = c.seg;
-        w.kvh = triple / p.head_tiles;
-        w.h0 = w.kvh * p.group + ht * A8_HEADS;
-        w.heads = min(A8_HEADS, p.group - ht * A8_HEADS);
-        w.pos = a8_pos(p, w.seg);
-        w.lo = a8_lo(p, w.pos);
-        w.tile = w.lo / A8_TILE + (lo_u - tile0);
-        w.ntiles = hi_u - lo_u;
-        w.whole = (lo_u == tile0 && hi_u == tile0 + n) ? 1 : 0;
-        w.slot = lo_u == tile0 ? 1 : 0;
-        w.cta_first = tile0 / c.span;
-        w.pieces = (tile0 + n - 1) / c.span - w.cta_first + 1;
-        c.f = hi_u;
-        return true;
-    }
-    return false;
+__device__ __forceinline__ bool a8_next(const A8Params& p, const A8Meta& meta, A8Cursor& c, A8Piece& w) {
+    if (c.f >= c.end) return false;
+    while (meta.pre[c.seg + 1] <= c.f) ++c.seg;                       // ends: f lies before the end of the sequence
+    const int first = meta.pre[c.seg];
+    w.pos = meta.pos[c.seg];
+    w.lo = a8_lo(p, w.pos);
+    const int n = w.pos / A8_TILE - w.lo / A8_TILE + 1, per = n + p.pair_cost;
+    const int triple = (c.f - first) / per;
+    const int unit0 = first + triple * per + p.pair_cost;             // unit of the triple's first tile
+    const int lo_u = max(c.f, unit0), hi_u = min(c.end, unit0 + n);
+    c.f = hi_u;
+    if (hi_u <= lo_u) { c.f = c.end; return false; }                  // the span ends among the cost units
+    w.kvh = p.head_tiles == 1 ? triple : triple / p.head_tiles;
+    const int ht = triple - w.kvh * p.head_tiles;
+    w.seg = c.seg;
+    w.slot = meta.slot[c.seg];
+    w.h0 = w.kvh * p.group + ht * A8_HEADS;
+    w.heads = min(A8_HEADS, p.group - ht * A8_HEADS);
+    w.tile = w.lo / A8_TILE + (lo_u - unit0);
+    w.ntiles = hi_u - lo_u;
+    w.unit0 = unit0; w.tiles = n;
+    w.begins = lo_u == unit0; w.ends = hi_u == unit0 + n;
+    return true;
 }
+
+// four elements of the result, at `at` in the output
+__device__ __forceinline__ void a8_write4(const A8Params& p, int row, size_t at, const float4& sum, float den) {
+    if (row < 0 || row >= p.num_tokens) return;
+    const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+    const __nv_bfloat162 a = __floats2bfloat162_rn(sum.x * inv, sum.y * inv), b = __floats2bfloat162_rn(sum.z * inv, sum.w * inv);
+    *reinterpret_cast<uint2*>(p.out + at) = make_uint2(*reinterpret_cast<const unsigned*>(&a), *reinterpret_cast<const unsigned*>(&b));
+}
+
+// a triple that was cut between warps or CTAs
+struct A8Join {
+    int first, which, stop;         // the CTA's warps that hold parts of it; the first one's lies in its slot `which`
+    int whole;                      // all of it lies in this CTA
+    int h0, heads, row;
+    int cta0, pieces;               // otherwise: the CTA it begins in, and how many it reaches into
+};
+
+// what a block keeps in shared memory
+template <int D>
+struct A8Shared {
+    static constexpr int LINE = D + 4;                    // floats of a head's line: no bank conflicts
+    static constexpr int HALF = 8 * D;                    // bytes of half a block: eight keys, or D / 2 lines of values
+    static constexpr int PITCH = HALF + 32;               // of the four in a unit: keeps value reads free of bank conflicts
+    static constexpr int UNIT = 4 * PITCH;
+    static constexpr int RING = A8_RING * 128 / D;        // units of the queue
+    static constexpr int TILES = 4;                       // tiles whose block numbers and scales are kept
+    alignas(16) unsigned char ring[A8_WARPS][RING * UNIT];   // the queue; afterwards the part of the triple that the warp began last
+    float part0[A8_WARPS][A8_HEADS][LINE];                // the part of the triple that began before the warp's span
+    float m[A8_WARPS * 2][A8_HEADS], l[A8_WARPS * 2][A8_HEADS];
+    int id[A8_WARPS][TILES][4];
+    float ks[A8_WARPS][TILES][4], vs[A8_WARPS][TILES][4];
+    unsigned long long bar[A8_WARPS][RING];               // a unit has arrived
+    A8Meta meta;
+    int scan[32];
+    A8Join join[A8_WARPS + 1];
+    int joins;                                            // of those that begin in the CTA
+    int cut[2];                                           // which join left its sum in workspace slot 0 and 1; -1: none
+    int last[2];
+
+    // accumulators of a part: which = 0 for a triple that began before the span of the warp, 1 for one that begins in it
+    __device__ __forceinline__ float* part(int warp, int which, int head) {
+        return which ? reinterpret_cast<float*>(ring[warp]) + head * LINE : part0[warp][head];
+    }
+};
 
 template <int D, bool E4M3>
 __global__ void __launch_bounds__(A8_THREADS, 1) attn_decode_8bit_kernel(const A8Params p) {
+    typedef A8Shared<D> Shared;
     constexpr int KC = D / 64;             // 16-byte pieces of a key row per lane
     constexpr int KS = D / 16;             // k steps of the first product, and 16-row tiles of V^T
-    constexpr int LINE = D + 4;            // floats of a head's line in shared memory: no bank conflicts
-    __shared__ int pre[2 * (A8_MAX_SEGS + 1)];
-    __shared__ float part_o[A8_WARPS][A8_HEADS][LINE];
-    __shared__ float part_m[A8_WARPS][A8_HEADS], part_l[A8_WARPS][A8_HEADS];
-    __shared__ int last_flag;
+    constexpr int RING = Shared::RING, UNIT = Shared::UNIT;
+    static_assert(Shared::RING * Shared::UNIT >= A8_HEADS * Shared::LINE * 4, "a part fits the queue");
+    extern __shared__ __align__(16) unsigned char a8_smem[];
+    Shared& sh = *reinterpret_cast<Shared*>(a8_smem);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const A8Meta& meta = sh.meta;
+    const unsigned bars = (unsigned)__cvta_generic_to_shared(sh.bar[warp]);
+    if (threadIdx.x < 2) sh.cut[threadIdx.x] = -1;
+    if (threadIdx.x == 0) { sh.joins = 0; sh.join[0].heads = 0; }
+    if (threadIdx.x < A8_WARPS * 2 * A8_HEADS) { (&sh.m[0][0])[threadIdx.x] = -INFINITY; (&sh.l[0][0])[threadIdx.x] = 0.0f; }
+    static_assert(A8_WARPS * 2 * A8_HEADS <= A8_THREADS, "one thread per entry");
+    if (lane < RING) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bars + 8 * lane) : "memory");
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     pdl_wait();
-    pdl_trigger(PDL_ATTENTION);
-    if (warp == 0) {
-        int run = 0, run_d = 0;
-        for (int s0 = 0; s0 < p.num_segments; s0 += 32) {
-            const int s = s0 + lane;
-            const int n = s < p.num_segments ? a8_seg_tiles(p, s) : 0, dflag = n > 0 ? 1 : 0;
-            int inc = n, inc_d = dflag;
+    const int page_blocks = 1 << (p.page_shift - 4);
+    {   // the segments' units, summed up by the whole block
+        const int triples = p.nkv * p.head_tiles;
+        const long long most = ((long long)p.bt_stride << p.page_shift) - 1;         // a position is kept within the block table
+        int run = 0;
+        for (int s0 = 0; s0 < p.num_segments; s0 += A8_THREADS) {
+            const int s = s0 + threadIdx.x;
+            int n = 0;
+            if (s < p.num_segments) {
+                const int len = p.seg_len[s], start = p.seg_start[s], slot = p.seg_slot[s], row = p.seg_off[s];
+                const int pos = (int)min((long long)start, most);
+                if (len == 1 && pos >= 0) n = triples * (pos / A8_TILE - a8_lo(p, pos) / A8_TILE + 1 + p.pair_cost);
+                sh.meta.pos[s] = pos; sh.meta.slot[s] = slot; sh.meta.row[s] = row;
+            }
+            int inc = n;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const int a = __shfl_up_sync(0xffffffffu, inc, o), b = __shfl_up_sync(0xffffffffu, inc_d, o);
-                if (lane >= o) { inc += a; inc_d += b; }
+                const int a = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += a;
             }
-            if (s < p.num_segments) { pre[s] = run + inc - n; pre[A8_MAX_SEGS + 1 + s] = run_d + inc_d - dflag; }
-            run += __shfl_sync(0xffffffffu, inc, 31);
-            run_d += __shfl_sync(0xffffffffu, inc_d, 31);
+            if (lane == 31) sh.scan[warp] = inc;
+            __syncthreads();
+            int before = run;
+#pragma unroll
+            for (int x = 0; x < A8_WARPS; ++x) {
+                const int sum = sh.scan[x];
+                if (x < warp) before += sum;
+                run += sum;
+            }
+            if (s < p.num_segments) sh.meta.pre[s] = before + inc - n;
+            if (s0 + A8_THREADS < p.num_segments) __syncthreads();
         }
-        if (lane == 0) { pre[p.num_segments] = run; pre[A8_MAX_SEGS + 1 + p.num_segments] = run_d; }
+        if (threadIdx.x == 0) sh.meta.pre[p.num_segments] = run;
     }
     __syncthreads();
-    A8Cursor cur;
-    a8_begin(p, pre, cur);
-    A8Piece w, cut[2];
-    int num_cut = 0;
-    const int page_blocks = 1 << (p.page_shift - 4);
-    while (a8_next(p, pre, cur, w)) {
-        const int slot = p.seg_slot[w.seg];
-        const bool has_row = slot >= 0 && slot < p.bt_rows;
-        const int* table = p.block_table + (size_t)(has_row ? slot : 0) * p.bt_stride;
-        // block (lane >> 3) of a tile: its number in the pool, -1 if it holds no visible key or has no page
-        auto lookup = [&](int tile) -> int {
-            const int key = tile * A8_TILE + (lane >> 3) * C8_BLOCK;
-            if (!has_row || tile >= w.tile + w.ntiles || key > w.pos || key + C8_BLOCK <= w.lo) return -1;
-            const int page = table[key >> p.page_shift];
-            if (page < 0 || page >= p.num_pages) return -1;
-            return (page * p.nkv + w.kvh) * page_blocks + ((key & ((1 << p.page_shift) - 1)) >> 4);
-        };
-        uint4 kr[4][2][KC], vr[KS][2];
-        float ks = 0.0f, vs = 0.0f, ks_next, vs_next;
-        auto load_k = [&](int id) {       // a block that is not there: block 0 is loaded and masked
-            const unsigned char* base = p.kcache + (size_t)max(id, 0) * (C8_BLOCK * D) + (g & 1) * D + 16 * t;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int c = 0; c < KC; ++c) kr[j][h][c] = a8_load(base + (4 * j + 2 * h) * D + 64 * c);
-        };
-        auto load_v = [&](int id) {       // id: of block t
-            const unsigned char* base = p.vcache + (size_t)max(id, 0) * (C8_BLOCK * D) + g * C8_BLOCK;
-#pragma unroll
-            for (int m = 0; m < KS; ++m)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) vr[m][h] = a8_load(base + (16 * m + 8 * h) * C8_BLOCK);
-        };
-        const int first = w.tile + warp, stop = w.tile + w.ntiles;
-        int id = lookup(first), id_next = lookup(first + A8_WARPS);
-        if (first < stop) {
-            load_k(id);
-            load_v(__shfl_sync(0xffffffffu, id, 8 * t));
-            ks = p.kscale[max(id, 0)]; vs = p.vscale[max(id, 0)];
+    // equal shares of all units for the CTAs (the first ones have one more where it does not come out even), and of a CTA's
+    // units for its warps
+    const int total = meta.pre[p.num_segments];
+    const int ctas = min((int)gridDim.x, (total + p.span_min - 1) / p.span_min);
+    if ((int)blockIdx.x >= ctas) return;
+    const A8Shares of_ctas(total, ctas);
+    const int cta_from = of_ctas.from(blockIdx.x), cta_len = of_ctas.from(blockIdx.x + 1) - cta_from;
+    const A8Shares of_warps(cta_len, A8_WARPS);
+
+    // ---- the queue: units K K V V of one tile after the other, piece after piece ------------------------------------
+    // Block numbers are looked up 32 at a time (lane = block, eight tiles), one batch ahead of use, the first ones of a piece
+    // while the piece before it is asked for: a look-up is two dependent loads, and a tile must not wait for them.
+    auto lookup = [&](const A8Piece& x, int tile) -> int {     // -1: a block without visible keys or without a page
+        const int key = tile * A8_TILE + lane * C8_BLOCK;
+        if (x.slot < 0 || x.slot >= p.bt_rows || key > x.pos || key + C8_BLOCK <= x.lo) return -1;
+        const int page = p.block_table[(size_t)x.slot * p.bt_stride + (key >> p.page_shift)];
+        if (page < 0 || page >= p.num_pages) return -1;
+        return (page * p.nkv + x.kvh) * page_blocks + ((key & ((1 << p.page_shift) - 1)) >> 4);
+    };
+    A8Cursor ahead;
+    A8Piece a, b;                                         // the piece whose tiles are being asked for, and the one behind it
+    a8_begin(p, meta, cta_from + of_warps.from(warp), cta_from + of_warps.from(warp + 1), ahead);
+    A8Cursor cur = ahead;
+    bool asking = a8_next(p, meta, ahead, a), more = asking && a8_next(p, meta, ahead, b);
+    int a_first = 0, a_done = 0, a_count = 0;             // first tile of the current batch, tiles of the piece asked for
+    int a_ids = -1, a_ids_next = -1, b_ids = -1;
+    if (asking) {
+        a_first = a.tile;
+        a_ids = lookup(a, a.tile);
+        a_ids_next = a.ntiles > 8 ? lookup(a, a.tile + 8) : -1;
+        if (more) b_ids = lookup(b, b.tile);
+    }
+    const unsigned ring = (unsigned)__cvta_generic_to_shared(sh.ring[warp]);
+    int put = 0, take = 0, phase = 0;                     // units to fill and to use next, parity of the latter
+    int pending = 0;                                      // units asked for and not used yet
+    bool ok = true;                                       // no wait has run out
+    // unit 0, 1: keys 8 unit .. + 7 of the four blocks; 2, 3: their lines (unit - 2) D / 2 .. of V^T.  Lane b < 4 copies block
+    // b; in the place of a block that is not there comes block 0, to be masked.
+    auto ask = [&](int unit) {
+        if (asking && ok) {
+            const int at4 = 4 * (a_done & 7);              // the tile's first block in the batch
+            const int id = __shfl_sync(0xffffffffu, a_ids, at4 + t);
+            if (unit == 0 && lane < 4) {
+                const int at = a_count & (Shared::TILES - 1);
+                sh.id[warp][at][lane] = id;
+                a8_copy4((unsigned)__cvta_generic_to_shared(&sh.ks[warp][at][lane]), p.kscale + max(id, 0));
+                a8_copy4((unsigned)__cvta_generic_to_shared(&sh.vs[warp][at][lane]), p.vscale + max(id, 0));
+            }
+            const unsigned bar = bars + 8 * put;
+            if (lane == 0) a8_expect(bar, 4 * Shared::HALF);
+            __syncwarp();                                  // the unit that lay here has been read by all lanes
+            ++pending;
+#ifdef A8_TEST_HOOKS
+            // test build: one copy is left out, so the wait for its unit runs out
+            const bool copies = lane < 4 && !(blockIdx.x == 0 && warp == 1 && a_count == 1 && unit == 2 && lane == 3);
+#else
+            const bool copies = lane < 4;
+#endif
+            if (copies)
+                a8_bulk(ring + put * UNIT + lane * Shared::PITCH,
+                        (unit < 2 ? p.kcache : p.vcache) + (size_t)max(id, 0) * (C8_BLOCK * D) + (unit & 1) * Shared::HALF, Shared::HALF, bar);
+            if (unit == 3) {                              // the next tile, or the next piece's first
+                ++a_count;
+                ++a_done;
+                if (a_done == a.ntiles) {
+                    a = b; a_done = 0; a_first = b.tile;
+                    a_ids = b_ids;
+                    asking = more;
+                    if (asking) {
+                        a_ids_next = a.ntiles > 8 ? lookup(a, a.tile + 8) : -1;
+                        more = a8_next(p, meta, ahead, b);
+                        if (more) b_ids = lookup(b, b.tile);
+                    }
+                } else if ((a_done & 7) == 0) {
+                    a_first += 8;
+                    a_ids = a_ids_next;
+                    a_ids_next = a_done + 8 < a.ntiles ? lookup(a, a_first + 8) : -1;
+                }
+            }
         }
+        if (unit == 0) a8_commit();                        // a group of scale copies per tile
+        put = put + 1 == RING ? 0 : put + 1;
+    };
+    // The next unit.  After a wait that ran out nothing more is asked for, the copies under way are still waited for (with the
+    // same limit), and the warp goes through the rest of its span without data.
+    auto arrived = [&]() {
+        if (pending > 0) {
+            const bool here = a8_arrived(bars + 8 * take, phase, 0x8b000000u | (blockIdx.x << 8) | (warp << 4) | take);
+            ok = __all_sync(0xffffffffu, here) && ok;
+        }
+    };
+    auto used = [&]() {
+        pending = max(0, pending - 1);
+        if (++take == RING) { take = 0; phase ^= 1; }
+    };
+#pragma unroll
+    for (int u = 0; u < RING; ++u) ask(u & 3);
+
+    int count = 0;
+    A8Piece w;
+    while (a8_next(p, meta, cur, w)) {
+        const int row = meta.row[w.seg];
         // queries of head g as the second operand, scaled by a power of two into [1, 2); lanes of heads that are not: zeros
         unsigned qb[KS][2];
         float f0, f1;
         {
-            const int row = p.seg_off[w.seg];
             const bool live = g < w.heads && row >= 0 && row < p.num_tokens;
             const bf16* src = p.q + (size_t)(live ? row : 0) * p.q_stride + (size_t)(w.h0 + (live ? g : 0)) * D + 16 * t;
             uint4 raw[KC][2];
@@ -253,30 +411,42 @@ __global__ void __launch_bounds__(A8_THREADS, 1) attn_decode_8bit_kernel(const A
         float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
 
 #pragma unroll 1
-        for (int tile = first; tile < stop; tile += A8_WARPS) {
-            const int id_after = lookup(tile + 2 * A8_WARPS);
-            const bool more = tile + A8_WARPS < stop;
-            ks_next = 0.0f; vs_next = 0.0f;
+        for (int tile = w.tile; tile < w.tile + w.ntiles; ++tile) {
             float s[4][4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                s[j][0] = 0.0f; s[j][1] = 0.0f; s[j][2] = 0.0f; s[j][3] = 0.0f;
+            for (int u = 0; u < 2; ++u) {
+                arrived();
+                uint4 kr[2][2][KC];
+                const unsigned char* rows = sh.ring[warp] + take * UNIT + (g >> 1) * Shared::PITCH + (g & 1) * D + 16 * t;
 #pragma unroll
-                for (int k = 0; k < KS; ++k) {
-                    unsigned a0, a1, a2, a3;
-                    c8_decode4<E4M3>(a8_word(kr[j][0][k / 4], k % 4), a0, a2);
-                    c8_decode4<E4M3>(a8_word(kr[j][1][k / 4], k % 4), a1, a3);
-                    a8_mma(s[j], a0, a1, a2, a3, qb[k][0], qb[k][1]);
-                }
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int c = 0; c < KC; ++c) kr[i][h][c] = *reinterpret_cast<const uint4*>(rows + (4 * i + 2 * h) * D + 64 * c);
+                used();
+                ask((u + RING) & 3);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) s[2 * u + i / 4][i % 4] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < KS; ++k)                 // two sums in turn: a product waits for the one before in its sum
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        unsigned a0, a1, a2, a3;
+                        c8_decode4<E4M3>(a8_word(kr[i][0][k / 4], k % 4), a0, a2);
+                        c8_decode4<E4M3>(a8_word(kr[i][1][k / 4], k % 4), a1, a3);
+                        a8_mma(s[2 * u + i], a0, a1, a2, a3, qb[k][0], qb[k][1]);
+                    }
             }
-            if (more) {
-                load_k(id_next);
-                ks_next = p.kscale[max(id_next, 0)]; vs_next = p.vscale[max(id_next, 0)];
-            }
+            const int at = count++ & (Shared::TILES - 1);
+            a8_wait_group<(RING + 1) / 4>();               // this tile's scales; those of the tiles asked for since may be under way
+            __syncwarp();
+            const int id = sh.id[warp][at][g >> 1];
+            const float ks = sh.ks[warp][at][g >> 1];
             // ---- softmax: all rows of a lane lie in block g >> 1 -------------------------------------------------
             const int base = tile * A8_TILE;
             const bool full = base >= w.lo && base + A8_TILE - 1 <= w.pos && __all_sync(0xffffffffu, id >= 0);
-            vs = fmaxf(vs, 8.673617379884035e-19f);      // 2^-60: a scale of zero still counts in the sum
+            const float vs = fmaxf(sh.vs[warp][at][g >> 1], 8.673617379884035e-19f);      // 2^-60: a scale of zero still counts in the sum
             const float lv = log2f(vs), c0 = f0 * ks, c1 = f1 * ks;
             float x0 = -INFINITY, x1 = -INFINITY;
 #pragma unroll
@@ -321,108 +491,198 @@ __global__ void __launch_bounds__(A8_THREADS, 1) attn_decode_8bit_kernel(const A
                     pb[j][h] = a8_turn(*reinterpret_cast<const unsigned*>(&v));
                 }
             l0 = fmaf(t0, back, l0); l1 = fmaf(t1, back, l1);
+            unsigned mask[4];
             if (!full) {                   // whatever lies in the value bytes of hidden keys must not meet a weight of zero
                 const int begin = base + t * C8_BLOCK;
                 const bool there = __shfl_sync(0xffffffffu, id, 8 * t) >= 0;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    unsigned mask = 0u;
+                    mask[j] = 0u;
 #pragma unroll
                     for (int b = 0; b < 4; ++b) {
                         const int key = begin + 4 * j + b;
-                        mask |= (there && key >= w.lo && key <= w.pos) ? 0xffu << (8 * b) : 0u;
+                        mask[j] |= (there && key >= w.lo && key <= w.pos) ? 0xffu << (8 * b) : 0u;
                     }
-#pragma unroll
-                    for (int m = 0; m < KS; ++m)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            if (j == 0) vr[m][h].x &= mask; else if (j == 1) vr[m][h].y &= mask;
-                            else if (j == 2) vr[m][h].z &= mask; else vr[m][h].w &= mask;
-                        }
                 }
             }
 #pragma unroll
-            for (int m = 0; m < KS; ++m) {
+            for (int u = 0; u < 2; ++u) {
+                arrived();
+                uint4 vr[KS / 2][2];
+                const unsigned char* lines = sh.ring[warp] + take * UNIT + t * Shared::PITCH + g * C8_BLOCK;
+#pragma unroll
+                for (int x = 0; x < KS; ++x) vr[x / 2][x % 2] = *reinterpret_cast<const uint4*>(lines + (x * 8) * C8_BLOCK);
+                used();
+                ask((u + 2 + RING) & 3);
+                if (!full) {
+#pragma unroll
+                    for (int x = 0; x < KS; ++x) {
+                        vr[x / 2][x % 2].x &= mask[0]; vr[x / 2][x % 2].y &= mask[1];
+                        vr[x / 2][x % 2].z &= mask[2]; vr[x / 2][x % 2].w &= mask[3];
+                    }
+                }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    unsigned a0, a1, a2, a3;
-                    c8_decode4<E4M3>(a8_word(vr[m][0], j), a0, a2);
-                    c8_decode4<E4M3>(a8_word(vr[m][1], j), a1, a3);
-                    a8_mma(o[m], a0, a1, a2, a3, pb[j][0], pb[j][1]);
+#pragma unroll
+                    for (int m = 0; m < KS / 2; ++m) {
+                        unsigned a0, a1, a2, a3;
+                        c8_decode4<E4M3>(a8_word(vr[m][0], j), a0, a2);
+                        c8_decode4<E4M3>(a8_word(vr[m][1], j), a1, a3);
+                        a8_mma(o[u * (KS / 2) + m], a0, a1, a2, a3, pb[j][0], pb[j][1]);
+                    }
                 }
             }
-            if (more) load_v(__shfl_sync(0xffffffffu, id_next, 8 * t));
-            id = id_next; id_next = id_after; ks = ks_next; vs = vs_next;
         }
-        // ---- the warps' shares of the piece, added up in warp order ---------------------------------------------------
+        // ---- the end of the piece -----------------------------------------------------------------------------------------
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) { l0 += __shfl_xor_sync(0xffffffffu, l0, d); l1 += __shfl_xor_sync(0xffffffffu, l1, d); }
-        if (g == 0) {
-            part_m[warp][2 * t] = m0; part_m[warp][2 * t + 1] = m1;
-            part_l[warp][2 * t] = l0; part_l[warp][2 * t + 1] = l1;
-        }
+        if (w.begins && w.ends) {                         // the whole triple
+            const float i0 = l0 == 0.0f ? 0.0f : 1.0f / l0, i1 = l1 == 0.0f ? 0.0f : 1.0f / l1;
+            const bool odd = (g & 1) != 0;                // lanes of neighbouring elements: the even one takes head 2t, the odd one 2t + 1
+            const int head = 2 * t + (odd ? 1 : 0);
+            bf16* dst = p.out + ((size_t)max(row, 0) * p.nq + w.h0 + head) * D + (g & ~1);
+            const bool write = row >= 0 && row < p.num_tokens && head < w.heads;
 #pragma unroll
-        for (int m = 0; m < KS; ++m) {
-            part_o[warp][2 * t][16 * m + g] = o[m][0]; part_o[warp][2 * t + 1][16 * m + g] = o[m][1];
-            part_o[warp][2 * t][16 * m + 8 + g] = o[m][2]; part_o[warp][2 * t + 1][16 * m + 8 + g] = o[m][3];
-        }
-        __syncthreads();
-        const int row = p.seg_off[w.seg];
-        for (int i = threadIdx.x; i < w.heads * D; i += A8_THREADS) {
-            const int h = i / D, e = i % D;
-            float top = -INFINITY, sum = 0.0f, den = 0.0f;
+            for (int m = 0; m < KS; ++m)
 #pragma unroll
-            for (int x = 0; x < A8_WARPS; ++x) top = fmaxf(top, part_m[x][h]);
+                for (int h = 0; h < 2; ++h) {
+                    const float a = o[m][2 * h] * i0, b = o[m][2 * h + 1] * i1;
+                    const float got = __shfl_xor_sync(0xffffffffu, odd ? a : b, 4);
+                    const __nv_bfloat162 v = odd ? __floats2bfloat162_rn(got, b) : __floats2bfloat162_rn(a, got);
+                    if (write) *reinterpret_cast<__nv_bfloat162*>(dst + 16 * m + 8 * h) = v;
+                }
+        } else {                                          // a part of one; one that begins here is the span's last piece
+            const int unit = w.unit0 + w.tile - w.lo / A8_TILE, last_unit = w.unit0 + w.tiles - 1;
+            if (lane == 0 && (w.begins || unit == cta_from)) {      // the triple's first part in this CTA: noted for the sum below
+                const int at = w.begins ? atomicAdd(&sh.joins, 1) + 1 : 0;
+                A8Join& j = sh.join[at];
+                j.first = warp; j.which = w.begins;
+                j.stop = last_unit < cta_from + cta_len ? of_warps.holds(last_unit - cta_from) : A8_WARPS - 1;
+                j.whole = w.begins && last_unit < cta_from + cta_len;
+                j.h0 = w.h0; j.heads = w.heads; j.row = row;
+                if (!j.whole) {
+                    j.cta0 = w.begins ? blockIdx.x : of_ctas.holds(w.unit0);
+                    j.pieces = of_ctas.holds(last_unit) - j.cta0 + 1;
+                }
+            }
+            const int part = warp * 2 + w.begins;
+            if (g == 0) {
+                sh.m[part][2 * t] = m0; sh.m[part][2 * t + 1] = m1;
+                sh.l[part][2 * t] = l0; sh.l[part][2 * t + 1] = l1;
+            }
+            float* p0 = sh.part(warp, w.begins, 2 * t);
+            float* p1 = sh.part(warp, w.begins, 2 * t + 1);
+            __syncwarp();                                 // the queue is no longer read
+#pragma unroll
+            for (int m = 0; m < KS; ++m) {
+                p0[16 * m + g] = o[m][0]; p1[16 * m + g] = o[m][1];
+                p0[16 * m + 8 + g] = o[m][2]; p1[16 * m + 8 + g] = o[m][3];
+            }
+        }
+    }
+    pdl_trigger();                         // all keys and values are in: the next kernel may take the memory system
+    __syncthreads();
+    // ---- triples that were cut between the warps of the CTA: their parts are added up in warp order.  Join 0 is a triple that
+    // began before the CTA, at most one of the others goes on behind it; these two leave their sum in the workspace -----------
+    const int joins = sh.joins + 1;
+    const int team = joins > A8_WARPS / 2 ? 1 : A8_WARPS / joins;                     // warps per triple
+    for (int at = warp / team; at < joins; at += A8_WARPS / team) {
+        const A8Join& j = sh.join[at];
+        if (j.heads == 0) continue;
+        for (int i = (warp % team) * 32 + lane; i < j.heads * (D / 4); i += team * 32) {
+            const int h = i / (D / 4), e = 4 * (i % (D / 4));
+            float f[A8_WARPS], top = -INFINITY, den = 0.0f;
+            float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            bool has[A8_WARPS];                               // a warp with an empty span, or without a visible key, has no part
+#pragma unroll
+            for (int x = 0; x < A8_WARPS; ++x) {
+                const int part = 2 * x + (x == j.first ? j.which : 0);
+                has[x] = x >= j.first && x <= j.stop && !(sh.m[part][h] == -INFINITY && sh.l[part][h] == 0.0f);
+                f[x] = has[x] ? sh.m[part][h] : -INFINITY;
+                top = fmaxf(top, f[x]);
+            }
             const float ref = top == -INFINITY ? 0.0f : top;
 #pragma unroll
             for (int x = 0; x < A8_WARPS; ++x) {
-                const float f = a8_ex2(part_m[x][h] - ref);
-                sum = fmaf(f, part_o[x][h][e], sum);
-                den = fmaf(f, part_l[x][h], den);
+                if (!has[x]) continue;
+                const int which = x == j.first ? j.which : 0;
+                const float wgt = a8_ex2(f[x] - ref);
+                const float4 v = *reinterpret_cast<const float4*>(sh.part(x, which, h) + e);
+                sum.x = fmaf(wgt, v.x, sum.x); sum.y = fmaf(wgt, v.y, sum.y); sum.z = fmaf(wgt, v.z, sum.z); sum.w = fmaf(wgt, v.w, sum.w);
+                den = fmaf(wgt, sh.l[2 * x + which][h], den);
             }
-            if (w.whole) {
-                if (row >= 0 && row < p.num_tokens)
-                    p.out[((size_t)row * p.nq + w.h0 + h) * D + e] = __float2bfloat16_rn(den == 0.0f ? 0.0f : sum / den);
+            if (j.whole) {
+                a8_write4(p, j.row, ((size_t)j.row * p.nq + j.h0 + h) * D + e, sum, den);
             } else {
-                const size_t at = ((size_t)blockIdx.x * 2 + w.slot) * A8_SLOT_HEADS + h;
-                p.ws_acc[at * D + e] = sum;
-                if (e == 0) { p.ws_ml[at * 2] = top; p.ws_ml[at * 2 + 1] = den; }
+                const size_t to = ((size_t)blockIdx.x * 2 + j.which) * A8_SLOT_HEADS + h;
+                *reinterpret_cast<float4*>(p.ws_acc + to * D + e) = sum;
+                if (e == 0) *reinterpret_cast<float2*>(p.ws_ml + to * 2) = make_float2(top, den);
             }
         }
-        if (!w.whole) cut[num_cut++] = w;
-        __syncthreads();
+        if (!j.whole && lane == 0 && warp % team == 0) sh.cut[j.which] = at;
     }
-    // ---- pieces of cut triples: reported when the span is done ---------------------------------------------------------
-    for (int c = 0; c < num_cut; ++c) {
-        const A8Piece& z = cut[c];
-        __threadfence();
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            const unsigned before = atomicAdd(&p.ws_count[z.cta_first], 1u);
-            last_flag = before + 1 == (unsigned)z.pieces;
-            if (last_flag) p.ws_count[z.cta_first] = 0u;          // zero for the next launch
+    // ---- triples that were cut between CTAs: the CTA that delivers the last piece adds them up in the order of the keys ------
+    __syncthreads();
+    if (threadIdx.x < 2) {
+        int last = 0;
+        if (sh.cut[threadIdx.x] >= 0) {
+            const A8Join& j = sh.join[sh.cut[threadIdx.x]];
+            __threadfence();                                  // the whole block's writes (the barrier above) before the count
+            last = atomicAdd(&p.ws_count[j.cta0], 1u) + 1 == (unsigned)j.pieces;
+            if (last) p.ws_count[j.cta0] = 0u;                // zero for the next launch
             __threadfence();
         }
-        __syncthreads();
-        if (!last_flag) continue;
-        const int row = p.seg_off[z.seg];
-        for (int i = threadIdx.x; i < z.heads * D; i += A8_THREADS) {
-            const int h = i / D, e = i % D;
-            float top = -INFINITY, sum = 0.0f, den = 0.0f;
-            for (int x = 0; x < z.pieces; ++x) {                  // the first piece lies in slot 1 of its CTA, the others in slot 0
-                const size_t at = ((size_t)(z.cta_first + x) * 2 + (x == 0 ? 1 : 0)) * A8_SLOT_HEADS + h;
-                const float m = __ldcg(&p.ws_ml[at * 2]), l = __ldcg(&p.ws_ml[at * 2 + 1]), a = __ldcg(&p.ws_acc[at * D + e]);
-                const float n = fmaxf(top, m), ref = n == -INFINITY ? 0.0f : n;
-                const float old = a8_ex2(top - ref), now = a8_ex2(m - ref);
-                sum = sum * old + a * now;
-                den = den * old + l * now;
-                top = n;
-            }
-            if (row >= 0 && row < p.num_tokens)
-                p.out[((size_t)row * p.nq + z.h0 + h) * D + e] = __float2bfloat16_rn(den == 0.0f ? 0.0f : sum / den);
-        }
-        __syncthreads();
+        sh.last[threadIdx.x] = last;
     }
+    __syncthreads();
+    constexpr int HALF_BLOCK = A8_THREADS / 2;                // one half of the block for each of the two
+    const int c = threadIdx.x / HALF_BLOCK;
+    if (!sh.last[c]) return;
+    const A8Join& j = sh.join[sh.cut[c]];
+    for (int i = threadIdx.x % HALF_BLOCK; i < j.heads * (D / 4); i += HALF_BLOCK) {
+        const int h = i / (D / 4), e = 4 * (i % (D / 4));
+        float top = -INFINITY, den = 0.0f;
+        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        constexpr int BATCH = 10;                             // pieces whose loads are in flight together
+        for (int x0 = 0; x0 < j.pieces; x0 += BATCH) {
+            float2 ml[BATCH];
+            float4 v[BATCH];
+#pragma unroll
+            for (int x = 0; x < BATCH; ++x) {
+                // the first piece lies in slot 1 of its CTA, the others in slot 0
+                const size_t at = ((size_t)(j.cta0 + min(x0 + x, j.pieces - 1)) * 2 + (x0 + x == 0 ? 1 : 0)) * A8_SLOT_HEADS + h;
+                ml[x] = __ldcg(reinterpret_cast<const float2*>(p.ws_ml) + at);
+                v[x] = __ldcg(reinterpret_cast<const float4*>(p.ws_acc + at * D + e));
+            }
+#pragma unroll
+            for (int x = 0; x < BATCH; ++x) {
+                if (x0 + x >= j.pieces) continue;
+                const float now = fmaxf(top, ml[x].x), ref = now == -INFINITY ? 0.0f : now;
+                const float old = a8_ex2(top - ref), wgt = a8_ex2(ml[x].x - ref);
+                sum.x = sum.x * old + v[x].x * wgt; sum.y = sum.y * old + v[x].y * wgt;
+                sum.z = sum.z * old + v[x].z * wgt; sum.w = sum.w * old + v[x].w * wgt;
+                den = den * old + ml[x].y * wgt;
+                top = now;
+            }
+        }
+        a8_write4(p, j.row, ((size_t)j.row * p.nq + j.h0 + h) * D + e, sum, den);
+    }
+}
+
+template <int D, bool E4M3>
+static int a8_launch(const A8Params& p, int ctas, cudaStream_t stream) {
+    const size_t smem = sizeof(A8Shared<D>);
+    static bool configured = false;
+    if (!configured) {
+        cudaError_t err = cudaFuncSetAttribute(attn_decode_8bit_kernel<D, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (err != cudaSuccess) {
+            snprintf(g_pi_error, sizeof(g_pi_error), "pi_attention_decode_8bit: cannot reserve %zu bytes of shared memory: %s", smem, cudaGetErrorString(err));
+            return (int)err;
+        }
+        configured = true;
+    }
+    pi_launch(attn_decode_8bit_kernel<D, E4M3>, dim3((unsigned)ctas), dim3(A8_THREADS), smem, stream, p);
+    return pi_check_launch("pi_attention_decode_8bit");
 }
 
 PI_EXPORT int pi_attention_decode_8bit(const void* q, int q_stride, const void* kcache, const void* vcache, const float* kscale,
@@ -439,7 +699,7 @@ PI_EXPORT int pi_attention_decode_8bit(const void* q, int q_stride, const void* 
     if (page_size < C8_BLOCK || (page_size & (page_size - 1))) return pi_refuse("pi_attention_decode_8bit: page size %d must be a power of two of at least 16", page_size);
     if (cache_dtype != PI_E4M3 && cache_dtype != PI_INT8) return pi_refuse("pi_attention_decode_8bit: unknown dtype code %d of the pages", cache_dtype);
     if (window < 0 || bt_rows <= 0 || bt_stride <= 0) return pi_refuse("pi_attention_decode_8bit: window=%d, block table [%d, %d]", window, bt_rows, bt_stride);
-    if (ws_ctas <= 0 || ws_acc == nullptr || ws_ml == nullptr || ws_count == nullptr) return pi_refuse("pi_attention_decode_8bit: the workspace is missing");
+    if (ws_ctas <= 0 || ws_ctas > 256 || ws_acc == nullptr || ws_ml == nullptr || ws_count == nullptr) return pi_refuse("pi_attention_decode_8bit: the workspace is missing (or for more than 256 CTAs: %d)", ws_ctas);
     if (span_min < 1 || pair_cost < 0 || pair_cost > 64) return pi_refuse("pi_attention_decode_8bit: span_min=%d must be at least 1 and pair_cost=%d between 0 and 64", span_min, pair_cost);
     if (q_stride % 8 != 0 || (((uintptr_t)q | (uintptr_t)kcache | (uintptr_t)vcache) & 15))
         return pi_refuse("pi_attention_decode_8bit: q and the pages must start on 16-byte boundaries, q with a stride that is a multiple of 8");
@@ -463,13 +723,18 @@ PI_EXPORT int pi_attention_decode_8bit(const void* q, int q_stride, const void* 
     if (window > 0 && seg_tiles > window / A8_TILE + 2) seg_tiles = window / A8_TILE + 2;
     const long long units = (long long)num_segments * nkv * p.head_tiles * (seg_tiles + pair_cost);
     if (units > 1000000000LL) return pi_refuse("pi_attention_decode_8bit: up to %lld tiles of keys are beyond the limit", units);
-    const dim3 grid((unsigned)ws_ctas), threads(A8_THREADS);
-    if (head_dim == 128) {
-        if (cache_dtype == PI_E4M3) pi_launch(attn_decode_8bit_kernel<128, true>, grid, threads, 0, stream, p);
-        else pi_launch(attn_decode_8bit_kernel<128, false>, grid, threads, 0, stream, p);
-    } else {
-        if (cache_dtype == PI_E4M3) pi_launch(attn_decode_8bit_kernel<64, true>, grid, threads, 0, stream, p);
-        else pi_launch(attn_decode_8bit_kernel<64, false>, grid, threads, 0, stream, p);
+    if (head_dim == 128) return cache_dtype == PI_E4M3 ? a8_launch<128, true>(p, ws_ctas, stream) : a8_launch<128, false>(p, ws_ctas, stream);
+    return cache_dtype == PI_E4M3 ? a8_launch<64, true>(p, ws_ctas, stream) : a8_launch<64, false>(p, ws_ctas, stream);
+}
+
+// 0 if every wait of the launches so far was met, else a code of the first that ran out (reading resets it)
+PI_EXPORT int pi_attention_8bit_status(unsigned* status) {
+    unsigned zero = 0;
+    cudaError_t err = cudaMemcpyFromSymbol(status, g_a8_status, sizeof(unsigned));
+    if (err == cudaSuccess) err = cudaMemcpyToSymbol(g_a8_status, &zero, sizeof(unsigned));
+    if (err != cudaSuccess) {
+        snprintf(g_pi_error, sizeof(g_pi_error), "pi_attention_8bit_status: %s", cudaGetErrorString(err));
+        return (int)err;
     }
-    return pi_check_launch("pi_attention_decode_8bit");
+    return 0;
 }

@@ -23,18 +23,15 @@ CACHE_8BIT_DTYPES = {torch.float8_e4m3fn: E4M3, torch.int8: INT8}
 PAGE_SIZES_8BIT = (16, 32, 64, 128)
 PAGE_MAPS_MAX_SEGMENTS = 4096
 _P, _I, _L, _F = _k.c_void_p, _k.c_int, _k.ctypes.c_longlong, _k.c_float
-_BOUND: dict = {}
 
 
 def _bound(library: str, name: str, argtypes: tuple):
-    """The C function with its argument types declared (plain Python numbers are then converted by ctypes itself)."""
-    held = _BOUND.get(name)
-    if held is None:
-        lib = _k._lib(library)
-        fn = getattr(lib, name)
-        fn.argtypes = list(argtypes)
-        held = _BOUND[name] = (lib, fn)
-    return held
+    """(library, C function) with its argument types declared: ctypes then converts plain Python numbers by itself."""
+    lib = _k._lib(library)
+    fn = getattr(lib, name)
+    if fn.argtypes is None:
+        fn.argtypes = argtypes
+    return lib, fn
 
 
 def _same_device(*tensors) -> None:
@@ -221,8 +218,8 @@ def pages_8bit_to_bf16(kcache: torch.Tensor, vcache: torch.Tensor, kscale: torch
 
 
 # ---- attention ----------------------------------------------------------------------------------------------------------
-DECODE_8BIT_SPAN_MIN = 8      # shortest span of a CTA in 64-key tiles and cost units: eight warps take a tile each
-DECODE_8BIT_PAIR_COST = 4     # units that a (request, kv head, eight query heads) triple counts for beside its tiles
+DECODE_8BIT_SPAN_MIN = 2      # shortest share of a CTA, in 64-key tiles and cost units
+DECODE_8BIT_PAIR_COST = 2     # units that a (request, kv head, eight query heads) triple counts for beside its tiles
 
 
 def _check_queries(what, q, q_stride, num_tokens, nq, nkv, d, window, scale, out) -> torch.Tensor:
@@ -308,3 +305,13 @@ def attention_prompt_8bit(q: torch.Tensor, q_stride: int, kcache: torch.Tensor, 
     return attention_tcgen05(q, q_stride, keys, values, maps.table, maps.seg_off, maps.rows, seg_start, seg_len, num_tokens, R,
                              longest, nq, nkv, d, page_size, window, scale, out, splits=splits, part_acc=acc, part_ml=ml,
                              token_seg=maps.token_seg)
+
+
+def attention_8bit_status() -> int:
+    """0 if every bounded wait of the decode kernel's launches so far was met (synchronises the device); 0 if it is not loaded."""
+    lib = _k._LIBS.get(("attention_8bit", None))
+    if lib is None:
+        return 0
+    status = _k.ctypes.c_uint(0)
+    _k._check(lib, lib.pi_attention_8bit_status(_k.ctypes.byref(status)), "attention_8bit_status", launches=0)
+    return int(status.value)
