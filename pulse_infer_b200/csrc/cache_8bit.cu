@@ -15,23 +15,30 @@
 // Not-a-number keys and values are stored as zero and infinities as the largest number of the format, so a page never
 // holds what would spread from a masked place (0 x NaN).
 //
-// One warp per (run, kv head, key or value): the scale needs the whole run, and a run is at most 16 rows of D elements -
-// 4 KB, held in registers.  Lanes of D / 8 form a group that takes 16-byte pieces of a row; a group takes consecutive
-// rows, so that for values its lanes hold consecutive bytes of the transposed block.  The warp of a token that does not
-// begin a run ends at once.  Query heads are plain streaming work, two rows in flight per group.
+// A block of four warps takes one key or value head of a run: the scale needs the whole run, at most 16 rows of D elements.
+// Lanes of D / 8 form a group that takes 16-byte pieces of one or two rows, so everything a run needs (rows, rotation, what lies
+// in the block) is asked for at once: the kernel is a chain of two round trips, the slots and the rest.  (One warp for all 16
+// rows went through the rotation tables of eight rows one after the other: 25 us instead of 12.)  A block looks for the
+// runs that begin among `window` tokens: 16 in a step of many tokens - one run, as a rule - and 1 in a decode step.  Query heads
+// are plain streaming work; in a step of many tokens they are a kernel of their own, in a small one part of the same launch.
+// Measured (B200, 32 + 8 + 8 heads of 128): 18 us for 2,045 tokens, both kernels, 46 MB (2.6 TB/s: too few loads in flight per
+// warp, as in the bf16 kernel); 2.9 us for 8 decoding requests.
 // ---------------------------------------------------------------------------------------------------
-#define CW_WARPS 8
-#define CW_Q_ROWS 2          // query rows in flight per lane group
+#define CW_WARPS 4
+#define CW_Q_ROWS 4          // query rows in flight per lane group
+#define CW_SMALL 128         // tokens up to which one launch does everything, a window of one token per block
 
 struct CwParams {
     const bf16* qkv; int row_stride;
-    const void* qw; const void* kw; float eps; int has_norm;
-    const float* cos_t; const float* sin_t; int rot_pairs, adjacent;
+    const void* qw; const void* kw; int wide; float eps; int has_norm;      // wide: the weights are float
+    const float* cos_t; const float* sin_t; int rot_pairs;
     unsigned char* kcache; unsigned char* vcache; float* kscale; float* vscale;
     const long long* slot_map; long long num_slots; int page_shift;
     bf16* q_out;
     int nq, nkv, num_tokens;
-    long long kv_units, q_units;      // warps' worth of work
+    int window;                       // tokens among which a block looks for the beginnings of runs: 1 or 16
+    long long kv_units;               // blocks' worth of keys and values
+    int q_shares;                     // warps' worth of a token's query heads
     int* error_count;
 };
 
@@ -49,9 +56,8 @@ __device__ __forceinline__ uint4 cw_pack(const float (&x)[8]) {
 }
 
 // 8 norm weights from element 8 * sub on
-template <typename TW>
-__device__ __forceinline__ void cw_weights(const void* w, int sub, float (&v)[8]) {
-    if constexpr (sizeof(TW) == 2) {
+__device__ __forceinline__ void cw_weights(const void* w, int wide, int sub, float (&v)[8]) {
+    if (!wide) {
         cw_unpack(reinterpret_cast<const uint4*>(w)[sub], v);
     } else {
         const float4 a = reinterpret_cast<const float4*>(w)[2 * sub], b = reinterpret_cast<const float4*>(w)[2 * sub + 1];
@@ -59,9 +65,34 @@ __device__ __forceinline__ void cw_weights(const void* w, int sub, float (&v)[8]
     }
 }
 
+// what the rotation of one row needs, for the 8 elements of a lane: asked for ahead of use
+template <bool ADJ> struct CwTurn { float c[ADJ ? 4 : 8], s[ADJ ? 4 : 8]; };
+
+template <int D, bool ADJ>
+__device__ __forceinline__ void cw_turn_load(const CwParams& p, int t, int sub, CwTurn<ADJ>& r) {
+    if (p.rot_pairs == 0) return;
+    const size_t row = (size_t)t * p.rot_pairs;
+    if constexpr (ADJ) {                                 // pairs (2i, 2i + 1); rot_pairs is a multiple of 4
+        if (4 * sub < p.rot_pairs) {
+            *reinterpret_cast<float4*>(r.c) = *reinterpret_cast<const float4*>(p.cos_t + row + 4 * sub);
+            *reinterpret_cast<float4*>(r.s) = *reinterpret_cast<const float4*>(p.sin_t + row + 4 * sub);
+        }
+    } else {                                            // pairs (i, i + rot_pairs); rot_pairs is a multiple of 8
+        const int shift = p.rot_pairs / 8;
+        if (sub < 2 * shift) {
+            const int at = 8 * (sub < shift ? sub : sub - shift);
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                *reinterpret_cast<float4*>(r.c + 4 * q) = *reinterpret_cast<const float4*>(p.cos_t + row + at + 4 * q);
+                *reinterpret_cast<float4*>(r.s + 4 * q) = *reinterpret_cast<const float4*>(p.sin_t + row + at + 4 * q);
+            }
+        }
+    }
+}
+
 // norm and rotation of one row spread over D / 8 lanes; every lane of the warp calls it (x of rows that do not exist: zeros)
-template <int D>
-__device__ __forceinline__ void cw_norm_rope(const CwParams& p, int t, int sub, const float (&w)[8], float (&x)[8]) {
+template <int D, bool ADJ>
+__device__ __forceinline__ void cw_norm_rope(const CwParams& p, int sub, const float (&w)[8], const CwTurn<ADJ>& r, float (&x)[8]) {
     constexpr int LANES = D / 8;
     if (p.has_norm) {
         float ss = 0.0f;
@@ -74,19 +105,15 @@ __device__ __forceinline__ void cw_norm_rope(const CwParams& p, int t, int sub, 
         for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * w[i];
     }
     if (p.rot_pairs == 0) return;
-    const size_t row = (size_t)t * p.rot_pairs;
-    if (p.adjacent) {                                   // pairs (2i, 2i + 1); rot_pairs is a multiple of 4
+    if constexpr (ADJ) {
         if (4 * sub < p.rot_pairs) {
-            const float4 c = *reinterpret_cast<const float4*>(p.cos_t + row + 4 * sub);
-            const float4 s = *reinterpret_cast<const float4*>(p.sin_t + row + 4 * sub);
-            const float cs[4] = {c.x, c.y, c.z, c.w}, sn[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
             for (int h = 0; h < 4; ++h) {
-                const float r0 = x[2 * h] * cs[h] - x[2 * h + 1] * sn[h], r1 = x[2 * h] * sn[h] + x[2 * h + 1] * cs[h];
+                const float r0 = x[2 * h] * r.c[h] - x[2 * h + 1] * r.s[h], r1 = x[2 * h] * r.s[h] + x[2 * h + 1] * r.c[h];
                 x[2 * h] = r0; x[2 * h + 1] = r1;
             }
         }
-    } else {                                            // pairs (i, i + rot_pairs); rot_pairs is a multiple of 8
+    } else {
         const int shift = p.rot_pairs / 8;              // the partner's lane
         const bool first = sub < shift, second = !first && sub < 2 * shift;
         const int partner = first ? sub + shift : second ? sub - shift : sub;
@@ -94,18 +121,8 @@ __device__ __forceinline__ void cw_norm_rope(const CwParams& p, int t, int sub, 
 #pragma unroll
         for (int i = 0; i < 8; ++i) other[i] = __shfl_sync(0xffffffffu, x[i], partner, LANES);
         if (first || second) {
-            const int at = 8 * (first ? sub : sub - shift);
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                const float4 c = *reinterpret_cast<const float4*>(p.cos_t + row + at + 4 * q);
-                const float4 s = *reinterpret_cast<const float4*>(p.sin_t + row + at + 4 * q);
-                const float cs[4] = {c.x, c.y, c.z, c.w}, sn[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-                for (int h = 0; h < 4; ++h) {
-                    const int i = 4 * q + h;
-                    x[i] = first ? x[i] * cs[h] - other[i] * sn[h] : other[i] * sn[h] + x[i] * cs[h];
-                }
-            }
+            for (int i = 0; i < 8; ++i) x[i] = first ? x[i] * r.c[i] - other[i] * r.s[i] : other[i] * r.s[i] + x[i] * r.c[i];
         }
     }
 }
@@ -116,79 +133,83 @@ __device__ __forceinline__ float cw_element(const uint4& raw, int i) {
     return __uint_as_float((i & 1) ? (w & 0xffff0000u) : (w << 16));
 }
 
-template <int D, typename TW, bool E4M3>
-__global__ void __launch_bounds__(CW_WARPS * 32) cache_8bit_write_kernel(const CwParams p) {
-    constexpr int LANES = D / 8, GROUPS = 32 / LANES, ROWS = C8_BLOCK / GROUPS;       // D 128: 2 groups of 8 rows; 64: 4 of 4
-    pdl_wait();
-    pdl_trigger();
+// query heads: a warp takes CW_Q_ROWS per lane group of one token, so that one piece of the rotation tables does for all
+template <int D, bool ADJ>
+__device__ __forceinline__ void cw_queries(const CwParams& p, unsigned unit) {
+    constexpr int LANES = D / 8, GROUPS = 32 / LANES;
     const int lane = threadIdx.x & 31, sub = lane % LANES, grp = lane / LANES;
-    const long long unit = (long long)blockIdx.x * CW_WARPS + (threadIdx.x >> 5);
-    if (unit >= p.kv_units) {
-        // ---- query rows: (token, head) pairs ------------------------------------------------------------------
-        const long long q_unit = unit - p.kv_units;
-        if (q_unit >= p.q_units) return;
-        float w[8];
-        if (p.has_norm) cw_weights<TW>(p.qw, sub, w);
-        uint4 raw[CW_Q_ROWS];
-        int tok[CW_Q_ROWS], head[CW_Q_ROWS];
-        const long long rows = (long long)p.num_tokens * p.nq;
+    const unsigned t = unit / (unsigned)p.q_shares;
+    if (t >= (unsigned)p.num_tokens) return;
+    const int head0 = (int)(unit - t * p.q_shares) * GROUPS * CW_Q_ROWS + grp;
+    const bf16* src = p.qkv + (size_t)t * p.row_stride;
+    bf16* dst = p.q_out + (size_t)t * p.nq * D;
+    uint4 raw[CW_Q_ROWS];
 #pragma unroll
-        for (int j = 0; j < CW_Q_ROWS; ++j) {
-            const long long row = (q_unit * CW_Q_ROWS + j) * GROUPS + grp;
-            tok[j] = row < rows ? (int)(row / p.nq) : -1;
-            head[j] = row < rows ? (int)(row - (long long)tok[j] * p.nq) : 0;
-            raw[j] = tok[j] >= 0 ? reinterpret_cast<const uint4*>(p.qkv + (size_t)tok[j] * p.row_stride + head[j] * D)[sub]
-                                 : make_uint4(0u, 0u, 0u, 0u);
-        }
+    for (int j = 0; j < CW_Q_ROWS; ++j)
+        raw[j] = head0 + j * GROUPS < p.nq ? reinterpret_cast<const uint4*>(src + (head0 + j * GROUPS) * D)[sub] : make_uint4(0u, 0u, 0u, 0u);
+    float w[8];
+    if (p.has_norm) cw_weights(p.qw, p.wide, sub, w);
+    CwTurn<ADJ> turn;
+    cw_turn_load<D, ADJ>(p, (int)t, sub, turn);
 #pragma unroll
-        for (int j = 0; j < CW_Q_ROWS; ++j) {
-            float x[8];
-            cw_unpack(raw[j], x);
-            cw_norm_rope<D>(p, max(tok[j], 0), sub, w, x);
-            if (tok[j] >= 0) reinterpret_cast<uint4*>(p.q_out + ((size_t)tok[j] * p.nq + head[j]) * D)[sub] = cw_pack(x);
-        }
-        return;
+    for (int j = 0; j < CW_Q_ROWS; ++j) {
+        float x[8];
+        cw_unpack(raw[j], x);
+        cw_norm_rope<D, ADJ>(p, sub, w, turn, x);
+        if (head0 + j * GROUPS < p.nq) reinterpret_cast<uint4*>(dst + (head0 + j * GROUPS) * D)[sub] = cw_pack(x);
     }
-    // ---- a run of tokens in one block of one key or value head ----------------------------------------------------
-    const int t = (int)(unit / (2 * p.nkv));
-    const int which = (int)(unit - (long long)t * 2 * p.nkv);
+}
+
+template <int D>
+struct CwShared {
+    float amax[CW_WARPS];
+    unsigned tile[D][5];          // a value block on its way to its transposed place: 16 bytes a line, padded
+};
+
+// the run of `count` tokens that begins with token t, in one block of one key or value head (which: key heads, then value
+// heads); the whole thread block
+template <int D, bool ADJ, bool E4M3>
+__device__ __forceinline__ void cw_run(const CwParams& p, CwShared<D>& sh, int t, long long slot, int count, int which) {
+    constexpr int LANES = D / 8, GROUPS = 32 / LANES, ROWS = C8_BLOCK / CW_WARPS / GROUPS;       // D 128: 2 rows a lane; 64: 1
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane % LANES, grp = lane / LANES;
     const bool is_v = which >= p.nkv;
     const int head = is_v ? which - p.nkv : which;
-    const long long slot = p.slot_map[t];
-    if (slot < 0 || slot >= p.num_slots) {
-        if (lane == 0) atomicAdd(p.error_count, 1);
-        return;
-    }
     const int off = (int)(slot & (C8_BLOCK - 1));
-    if (off != 0 && t > 0 && p.slot_map[t - 1] == slot - 1) return;                    // its run began earlier
-    int count;
-    {
-        const bool member = lane < C8_BLOCK - off && t + lane < p.num_tokens && p.slot_map[t + lane] == slot + lane;
-        count = __ffs(~__ballot_sync(0xffffffffu, member)) - 1;                        // at least 1
-    }
     const int page_blocks = 1 << (p.page_shift - 4);
     const long long page = slot >> p.page_shift;
     const long long block = (page * p.nkv + head) * page_blocks + (((int)slot & ((1 << p.page_shift) - 1)) >> 4);
     unsigned char* data = (is_v ? p.vcache : p.kcache) + (size_t)block * C8_BLOCK * D;
     float* scale = (is_v ? p.vscale : p.kscale) + block;
+    const int row0 = (warp * GROUPS + grp) * ROWS;                                      // the lane's rows of the block
 
-    // the new rows, in bf16, and their largest magnitude
+    // everything that is read, at once
     const bf16* src = p.qkv + (size_t)t * p.row_stride + (size_t)(p.nq + which) * D;
     uint4 row[ROWS];
+    CwTurn<ADJ> turn[ROWS];
+    uint2 old_k[ROWS];
+    uint4 old_v = make_uint4(0u, 0u, 0u, 0u);
+    const float old_scale = off > 0 ? *scale : 0.0f;
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
-        const int i = grp * ROWS + r - off;                                             // token t + i
-        row[r] = (i >= 0 && i < count) ? reinterpret_cast<const uint4*>(src + (size_t)i * p.row_stride)[sub] : make_uint4(0u, 0u, 0u, 0u);
+        const int i = row0 + r - off;                                                   // token t + i
+        const bool fresh = i >= 0 && i < count;
+        row[r] = fresh ? reinterpret_cast<const uint4*>(src + (size_t)i * p.row_stride)[sub] : make_uint4(0u, 0u, 0u, 0u);
+        old_k[r] = make_uint2(0u, 0u);
+        if (!is_v) {
+            cw_turn_load<D, ADJ>(p, t + max(0, min(i, count - 1)), sub, turn[r]);
+            if (!fresh && off > 0) old_k[r] = reinterpret_cast<const uint2*>(data + (row0 + r) * D)[sub];
+        }
     }
+    if (is_v && off > 0 && threadIdx.x < D) old_v = reinterpret_cast<const uint4*>(data)[threadIdx.x];
     if (!is_v) {
         float w[8];
-        if (p.has_norm) cw_weights<TW>(p.kw, sub, w);
+        if (p.has_norm) cw_weights(p.kw, p.wide, sub, w);
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
-            const int i = grp * ROWS + r - off;
+            const int i = row0 + r - off;
             float x[8];
             cw_unpack(row[r], x);
-            cw_norm_rope<D>(p, t + max(0, min(i, count - 1)), sub, w, x);
+            cw_norm_rope<D, ADJ>(p, sub, w, turn[r], x);
             if (i >= 0 && i < count) row[r] = cw_pack(x);
         }
     }
@@ -199,81 +220,125 @@ __global__ void __launch_bounds__(CW_WARPS * 32) cache_8bit_write_kernel(const C
         for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(cw_element(row[r], i)));     // fmaxf passes over NaN
     }
     amax = warp_max(amax);
+    if (lane == 0) sh.amax[warp] = amax;
+    __syncthreads();                                      // (also: every thread has read the old scale)
+#pragma unroll
+    for (int x = 0; x < CW_WARPS; ++x) amax = fmaxf(amax, sh.amax[x]);
     int e = c8_exponent<E4M3>(amax), e_old = e;
-    if (off > 0) { e_old = c8_scale_exponent(*scale); e = max(e, e_old); }
+    if (off > 0) { e_old = c8_scale_exponent(old_scale); e = max(e, e_old); }
     const bool again = off > 0 && e != e_old;             // what lies in the block is encoded again
     const float inv = c8_pow2(-e), shrink = c8_pow2(e_old - e);
-    __syncwarp();
-    if (lane == 0 && (off == 0 || again)) *scale = c8_pow2(e);
+    if (threadIdx.x == 0 && (off == 0 || again)) *scale = c8_pow2(e);
     auto coded = [&](float a, float b) -> unsigned {
         a = a == a ? a * inv : 0.0f;
         b = b == b ? b * inv : 0.0f;
         return c8_encode2<E4M3>(a, b);
     };
-    auto shrunk = [&](unsigned codes) -> unsigned {       // two old codes at the new scale
-        const float2 v = __half22float2(c8_decode2<E4M3>(codes));
-        return c8_encode2<E4M3>(v.x * shrink, v.y * shrink);
+    auto shrunk = [&](unsigned codes) -> unsigned {       // four old codes at the new scale
+        const float2 a = __half22float2(c8_decode2<E4M3>(codes & 0xffffu)), b = __half22float2(c8_decode2<E4M3>(codes >> 16));
+        return c8_encode2<E4M3>(a.x * shrink, a.y * shrink) | (c8_encode2<E4M3>(b.x * shrink, b.y * shrink) << 16);
     };
+    uint2 code[ROWS];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+        code[r].x = coded(cw_element(row[r], 0), cw_element(row[r], 1)) | (coded(cw_element(row[r], 2), cw_element(row[r], 3)) << 16);
+        code[r].y = coded(cw_element(row[r], 4), cw_element(row[r], 5)) | (coded(cw_element(row[r], 6), cw_element(row[r], 7)) << 16);
+    }
     if (!is_v) {
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
-            const int at = grp * ROWS + r, i = at - off;
+            const int i = row0 + r - off;
             const bool fresh = i >= 0 && i < count;
-            if (!fresh && off > 0 && !again) continue;
-            uint2* dst = reinterpret_cast<uint2*>(data + at * D) + sub;
-            uint2 out = make_uint2(0u, 0u);
-            if (fresh) {
-                out.x = coded(cw_element(row[r], 0), cw_element(row[r], 1)) | (coded(cw_element(row[r], 2), cw_element(row[r], 3)) << 16);
-                out.y = coded(cw_element(row[r], 4), cw_element(row[r], 5)) | (coded(cw_element(row[r], 6), cw_element(row[r], 7)) << 16);
-            } else if (off > 0) {
-                const uint2 old = *dst;
-                out.x = shrunk(old.x & 0xffffu) | (shrunk(old.x >> 16) << 16);
-                out.y = shrunk(old.y & 0xffffu) | (shrunk(old.y >> 16) << 16);
-            }
-            *dst = out;
+            if (!fresh && off > 0 && !again) continue;    // stays as it is
+            reinterpret_cast<uint2*>(data + (row0 + r) * D)[sub] = fresh ? code[r] : off > 0 ? make_uint2(shrunk(old_k[r].x), shrunk(old_k[r].y)) : make_uint2(0u, 0u);
         }
     } else {
-        // element i of the lane's rows: ROWS consecutive bytes of line 8 sub + i of the transposed block
-        const int lo = grp * ROWS - off;                  // token (counted from t) of the lane's first row
-        const bool any_fresh = lo < count && lo + ROWS > 0;
-        if (!any_fresh && off > 0 && !again) return;
+        unsigned char* tile = reinterpret_cast<unsigned char*>(sh.tile);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            unsigned* dst = reinterpret_cast<unsigned*>(data + (8 * sub + i) * C8_BLOCK + grp * ROWS);
+        for (int r = 0; r < ROWS; ++r)
 #pragma unroll
-            for (int q = 0; q < ROWS / 4; ++q) {
-                unsigned old = 0u;
-                if (off > 0) {
-                    old = dst[q];
-                    if (again) old = shrunk(old & 0xffffu) | (shrunk(old >> 16) << 16);
-                }
-                const unsigned fresh = coded(cw_element(row[4 * q], i), cw_element(row[4 * q + 1], i)) |
-                                       (coded(cw_element(row[4 * q + 2], i), cw_element(row[4 * q + 3], i)) << 16);
+            for (int i = 0; i < 8; ++i) tile[(8 * sub + i) * 20 + row0 + r] = (unsigned char)((i < 4 ? code[r].x : code[r].y) >> (8 * (i & 3)));
+        __syncthreads();
+        if (threadIdx.x < D) {                            // a line of 16 tokens
+            unsigned o[4] = {old_v.x, old_v.y, old_v.z, old_v.w};
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
                 unsigned mask = 0u;
 #pragma unroll
-                for (int b = 0; b < 4; ++b) mask |= (lo + 4 * q + b >= 0 && lo + 4 * q + b < count) ? 0xffu << (8 * b) : 0u;
-                dst[q] = (fresh & mask) | (old & ~mask);
+                for (int b = 0; b < 4; ++b) mask |= (4 * q + b >= off && 4 * q + b < off + count) ? 0xffu << (8 * b) : 0u;
+                if (again) o[q] = shrunk(o[q]);
+                o[q] = (sh.tile[threadIdx.x][q] & mask) | (o[q] & ~mask);
             }
+            reinterpret_cast<uint4*>(data)[threadIdx.x] = make_uint4(o[0], o[1], o[2], o[3]);
         }
     }
 }
 
-template <int D>
-static int cw_launch(const CwParams& p, int weight_dtype, int code, cudaStream_t stream) {
+template <int D, bool ADJ, bool E4M3, bool QUERIES>
+__global__ void __launch_bounds__(CW_WARPS * 32, 6) cache_8bit_write_kernel(const CwParams p) {
+    __shared__ CwShared<D> sh;
+    static_assert(CW_WARPS * 32 >= D, "a thread for each line of a value block");
+    pdl_wait();
+    pdl_trigger();
+    const int lane = threadIdx.x & 31;
+    const long long unit = blockIdx.x;
+    if (unit >= p.kv_units) {
+        if (QUERIES) cw_queries<D, ADJ>(p, (unsigned)(unit - p.kv_units) * CW_WARPS + (threadIdx.x >> 5));
+        return;
+    }
+    const int first = (int)(unit / (2 * p.nkv)) * p.window;
+    const int which = (int)(unit % (2 * p.nkv));
+    // lane i: token first + i.  A run that begins in the window ends within 15 more tokens.
+    const int mine = first + lane;
+    const long long slot = mine < p.num_tokens ? p.slot_map[mine] : -1;
+    long long before = __shfl_up_sync(0xffffffffu, slot, 1);
+    if (lane == 0) before = first > 0 ? p.slot_map[first - 1] : -1;
+    const bool there = slot >= 0 && slot < p.num_slots, in_window = lane < p.window && mine < p.num_tokens;
+    if (in_window && !there && threadIdx.x < 32) atomicAdd(p.error_count, 1);
+    // a token begins a run if the one before it does not lie just before it in the same block
+    unsigned begins = __ballot_sync(0xffffffffu, in_window && there && ((slot & (C8_BLOCK - 1)) == 0 || before != slot - 1));
+    while (begins != 0u) {                                   // the same in all warps
+        const int i = __ffs(begins) - 1;
+        begins &= begins - 1;
+        const long long start = __shfl_sync(0xffffffffu, slot, i);
+        const int room = C8_BLOCK - (int)(start & (C8_BLOCK - 1));
+        const unsigned members = __ballot_sync(0xffffffffu, lane >= i && lane < i + room && slot == start + (lane - i)) >> i;
+        cw_run<D, ADJ, E4M3>(p, sh, first + i, start, __ffs(~members) - 1, which);
+        if (begins != 0u) __syncthreads();
+    }
+}
+
+template <int D, bool ADJ>
+__global__ void __launch_bounds__(CW_WARPS * 32) cache_8bit_queries_kernel(const CwParams p) {
+    pdl_wait();
+    pdl_trigger();
+    cw_queries<D, ADJ>(p, blockIdx.x * CW_WARPS + (threadIdx.x >> 5));
+}
+
+template <int D, bool ADJ>
+static int cw_launch(const CwParams& p, int code, int* launches, cudaStream_t stream) {
     constexpr int GROUPS = 32 / (D / 8);
     CwParams q = p;
-    q.kv_units = (long long)p.num_tokens * 2 * p.nkv;
-    q.q_units = ((long long)p.num_tokens * p.nq + GROUPS * CW_Q_ROWS - 1) / (GROUPS * CW_Q_ROWS);
-    const long long blocks = (q.kv_units + q.q_units + CW_WARPS - 1) / CW_WARPS;
-    if (blocks > 2147483647LL) return pi_refuse("pi_cache_8bit_write: %d tokens are beyond the grid limit", p.num_tokens);
-    const dim3 grid((unsigned)blocks), threads(CW_WARPS * 32);
-    const bool wide = weight_dtype == PI_F32;
-    if (code == PI_E4M3) {
-        if (wide) pi_launch(cache_8bit_write_kernel<D, float, true>, grid, threads, 0, stream, q);
-        else pi_launch(cache_8bit_write_kernel<D, bf16, true>, grid, threads, 0, stream, q);
+    const bool small = p.num_tokens <= CW_SMALL;
+    q.window = small ? 1 : C8_BLOCK;
+    q.kv_units = ((long long)p.num_tokens + q.window - 1) / q.window * 2 * p.nkv;
+    q.q_shares = max(1, (p.nq + GROUPS * CW_Q_ROWS - 1) / (GROUPS * CW_Q_ROWS));
+    const long long q_units = p.nq > 0 ? (long long)p.num_tokens * q.q_shares : 0;
+    const long long q_blocks = (q_units + CW_WARPS - 1) / CW_WARPS, kv_blocks = q.kv_units + (small ? q_blocks : 0);
+    if (kv_blocks > 2147483647LL || q_units > 2147483647LL) return pi_refuse("pi_cache_8bit_write: %d tokens are beyond the grid limit", p.num_tokens);
+    const dim3 threads(CW_WARPS * 32);
+    *launches = 1;
+    if (!small && q_blocks > 0) {
+        pi_launch(cache_8bit_queries_kernel<D, ADJ>, dim3((unsigned)q_blocks), threads, 0, stream, q);
+        *launches = 2;
+    }
+    const dim3 grid((unsigned)kv_blocks);
+    if (small) {
+        if (code == PI_E4M3) pi_launch(cache_8bit_write_kernel<D, ADJ, true, true>, grid, threads, 0, stream, q);
+        else pi_launch(cache_8bit_write_kernel<D, ADJ, false, true>, grid, threads, 0, stream, q);
     } else {
-        if (wide) pi_launch(cache_8bit_write_kernel<D, float, false>, grid, threads, 0, stream, q);
-        else pi_launch(cache_8bit_write_kernel<D, bf16, false>, grid, threads, 0, stream, q);
+        if (code == PI_E4M3) pi_launch(cache_8bit_write_kernel<D, ADJ, true, false>, grid, threads, 0, stream, q);
+        else pi_launch(cache_8bit_write_kernel<D, ADJ, false, false>, grid, threads, 0, stream, q);
     }
     return pi_check_launch("pi_cache_8bit_write");
 }
@@ -282,7 +347,8 @@ PI_EXPORT int pi_cache_8bit_write(const void* qkv, int row_stride, const void* q
                                   float eps, int has_norm, const float* cos_t, const float* sin_t, int rot_pairs, int adjacent,
                                   void* kcache, void* vcache, float* kscale, float* vscale, int cache_dtype, long long num_pages,
                                   int page_size, const long long* slot_map, void* q_out, int nq, int nkv, int head_dim,
-                                  int num_tokens, int* error_count, cudaStream_t stream) {
+                                  int num_tokens, int* error_count, int* launches, cudaStream_t stream) {
+    *launches = 0;
     if (num_tokens <= 0) return 0;
     if (head_dim != 64 && head_dim != 128) return pi_refuse("pi_cache_8bit_write: head size %d is not 64 or 128", head_dim);
     if (nq < 0 || nkv <= 0) return pi_refuse("pi_cache_8bit_write: nq=%d nkv=%d", nq, nkv);
@@ -298,13 +364,15 @@ PI_EXPORT int pi_cache_8bit_write(const void* qkv, int row_stride, const void* q
         return pi_refuse("pi_cache_8bit_write: tensors must start on 16-byte boundaries");
     CwParams p;
     p.qkv = (const bf16*)qkv; p.row_stride = row_stride; p.qw = q_weight; p.kw = k_weight; p.eps = eps; p.has_norm = has_norm;
-    p.cos_t = cos_t; p.sin_t = sin_t; p.rot_pairs = rot_pairs; p.adjacent = adjacent;
+    p.cos_t = cos_t; p.sin_t = sin_t; p.rot_pairs = rot_pairs;
     p.kcache = (unsigned char*)kcache; p.vcache = (unsigned char*)vcache; p.kscale = kscale; p.vscale = vscale;
     p.slot_map = slot_map; p.num_slots = num_pages * page_size; p.page_shift = 0;
     while ((1 << p.page_shift) < page_size) ++p.page_shift;
     p.q_out = (bf16*)q_out; p.nq = nq; p.nkv = nkv; p.num_tokens = num_tokens; p.error_count = error_count;
-    p.kv_units = p.q_units = 0;
-    return head_dim == 128 ? cw_launch<128>(p, weight_dtype, cache_dtype, stream) : cw_launch<64>(p, weight_dtype, cache_dtype, stream);
+    p.kv_units = 0; p.window = p.q_shares = 1; p.wide = weight_dtype == PI_F32;
+    if (adjacent)
+        return head_dim == 128 ? cw_launch<128, true>(p, cache_dtype, launches, stream) : cw_launch<64, true>(p, cache_dtype, launches, stream);
+    return head_dim == 128 ? cw_launch<128, false>(p, cache_dtype, launches, stream) : cw_launch<64, false>(p, cache_dtype, launches, stream);
 }
 
 // ---------------------------------------------------------------------------------------------------

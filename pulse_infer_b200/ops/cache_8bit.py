@@ -181,13 +181,15 @@ def qk_norm_rope_write_8bit(qkv: torch.Tensor, q_weight, k_weight, eps: float, c
     elif q_out.dtype != torch.bfloat16 or tuple(q_out.shape) != (T, nq * d) or not q_out.is_contiguous():
         raise KernelError(f"q_out must be contiguous bfloat16 [{T}, {nq * d}]")
     lib, fn = _bound("cache_8bit", "pi_cache_8bit_write",
-                     (_P, _I, _P, _P, _I, _F, _I, _P, _P, _I, _I, _P, _P, _P, _P, _I, _L, _I, _P, _P, _I, _I, _I, _I, _P, _P))
+                     (_P, _I, _P, _P, _I, _F, _I, _P, _P, _I, _I, _P, _P, _P, _P, _I, _L, _I, _P, _P, _I, _I, _I, _I, _P, _P, _P))
+    launched = _I(0)
     _k._check(lib, fn(qkv.data_ptr(), qkv.stride(0) if T > 1 else qkv.shape[1], q_weight.data_ptr() if has_norm else None,
                       k_weight.data_ptr() if has_norm else None, _k._code(q_weight.dtype) if has_norm else BF16, eps,
                       1 if has_norm else 0, cos.data_ptr() if rot_pairs else None, sin.data_ptr() if rot_pairs else None,
                       rot_pairs, 1 if adjacent_pairs else 0, kcache.data_ptr(), vcache.data_ptr(), kscale.data_ptr(),
                       vscale.data_ptr(), code, pages, page_size, slot_map.data_ptr(), q_out.data_ptr(), nq, nkv, d, T,
-                      error_count.data_ptr(), _k._stream()), "qk_norm_rope_write_8bit")
+                      error_count.data_ptr(), _k.ctypes.byref(launched), _k._stream()), "qk_norm_rope_write_8bit", launches=0)
+    _k.count_launches(launched.value)
     return q_out
 
 
