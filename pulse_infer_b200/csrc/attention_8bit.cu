@@ -685,12 +685,23 @@ static int a8_launch(const A8Params& p, int ctas, cudaStream_t stream) {
     return pi_check_launch("pi_attention_decode_8bit");
 }
 
-PI_EXPORT int pi_attention_decode_8bit(const void* q, int q_stride, const void* kcache, const void* vcache, const float* kscale,
-                                       const float* vscale, int cache_dtype, long long num_pages, const int* block_table, int bt_rows,
-                                       int bt_stride, const int* seg_off, const int* seg_slot, const int* seg_start,
-                                       const int* seg_len, void* out, float* ws_acc, float* ws_ml, void* ws_count, int ws_ctas,
-                                       int span_min, int pair_cost, int num_tokens, int num_segments, int nq, int nkv, int head_dim,
-                                       int page_size, int window, float scale, cudaStream_t stream) {
+// arguments as one record of 8-byte fields
+struct A8Args {
+    const void* q; long long q_stride; const void* kcache; const void* vcache; const float* kscale; const float* vscale;
+    long long cache_dtype, num_pages; const int* block_table; long long bt_rows, bt_stride;
+    const int* seg_off; const int* seg_slot; const int* seg_start; const int* seg_len; void* out;
+    float* ws_acc; float* ws_ml; void* ws_count; long long ws_ctas, span_min, pair_cost;
+    long long num_tokens, num_segments, nq, nkv, head_dim, page_size, window;
+    double scale;
+};
+
+PI_EXPORT int pi_attention_decode_8bit(const A8Args* args, cudaStream_t stream) {
+    const A8Args& a = *args;
+    const int q_stride = (int)a.q_stride, cache_dtype = (int)a.cache_dtype, bt_rows = (int)a.bt_rows, bt_stride = (int)a.bt_stride;
+    const int ws_ctas = (int)a.ws_ctas, span_min = (int)a.span_min, pair_cost = (int)a.pair_cost, num_tokens = (int)a.num_tokens;
+    const int num_segments = (int)a.num_segments, nq = (int)a.nq, nkv = (int)a.nkv, head_dim = (int)a.head_dim;
+    const int page_size = (int)a.page_size, window = (int)a.window;
+    const float scale = (float)a.scale;
     if (num_segments <= 0 || num_tokens <= 0) return 0;
     if (head_dim != 64 && head_dim != 128) return pi_refuse("pi_attention_decode_8bit: head size %d is not 64 or 128", head_dim);
     if (!(scale > 0.0f)) return pi_refuse("pi_attention_decode_8bit: the score scale must be positive");
@@ -699,21 +710,21 @@ PI_EXPORT int pi_attention_decode_8bit(const void* q, int q_stride, const void* 
     if (page_size < C8_BLOCK || (page_size & (page_size - 1))) return pi_refuse("pi_attention_decode_8bit: page size %d must be a power of two of at least 16", page_size);
     if (cache_dtype != PI_E4M3 && cache_dtype != PI_INT8) return pi_refuse("pi_attention_decode_8bit: unknown dtype code %d of the pages", cache_dtype);
     if (window < 0 || bt_rows <= 0 || bt_stride <= 0) return pi_refuse("pi_attention_decode_8bit: window=%d, block table [%d, %d]", window, bt_rows, bt_stride);
-    if (ws_ctas <= 0 || ws_ctas > 256 || ws_acc == nullptr || ws_ml == nullptr || ws_count == nullptr) return pi_refuse("pi_attention_decode_8bit: the workspace is missing (or for more than 256 CTAs: %d)", ws_ctas);
+    if (ws_ctas <= 0 || ws_ctas > 256 || a.ws_acc == nullptr || a.ws_ml == nullptr || a.ws_count == nullptr) return pi_refuse("pi_attention_decode_8bit: the workspace is missing (or for more than 256 CTAs: %d)", ws_ctas);
     if (span_min < 1 || pair_cost < 0 || pair_cost > 64) return pi_refuse("pi_attention_decode_8bit: span_min=%d must be at least 1 and pair_cost=%d between 0 and 64", span_min, pair_cost);
-    if (q_stride % 8 != 0 || (((uintptr_t)q | (uintptr_t)kcache | (uintptr_t)vcache) & 15))
+    if (q_stride % 8 != 0 || (((uintptr_t)a.q | (uintptr_t)a.kcache | (uintptr_t)a.vcache) & 15))
         return pi_refuse("pi_attention_decode_8bit: q and the pages must start on 16-byte boundaries, q with a stride that is a multiple of 8");
-    const long long blocks = num_pages * nkv * (page_size / C8_BLOCK);
-    if (num_pages <= 0 || blocks > 2147483647LL) return pi_refuse("pi_attention_decode_8bit: %lld pages are %lld blocks: beyond the limit", num_pages, blocks);
+    const long long blocks = a.num_pages * nkv * (page_size / C8_BLOCK);
+    if (a.num_pages <= 0 || blocks > 2147483647LL) return pi_refuse("pi_attention_decode_8bit: %lld pages are %lld blocks: beyond the limit", a.num_pages, blocks);
     if ((long long)bt_stride * page_size > 2147483647LL - 2 * A8_TILE * A8_WARPS * 4)
         return pi_refuse("pi_attention_decode_8bit: block tables of %d pages are beyond the limit", bt_stride);
     A8Params p;
-    p.q = (const bf16*)q; p.q_stride = q_stride;
-    p.kcache = (const unsigned char*)kcache; p.vcache = (const unsigned char*)vcache; p.kscale = kscale; p.vscale = vscale;
-    p.block_table = block_table; p.bt_rows = bt_rows; p.bt_stride = bt_stride;
-    p.seg_off = seg_off; p.seg_slot = seg_slot; p.seg_start = seg_start; p.seg_len = seg_len;
-    p.out = (bf16*)out; p.ws_acc = ws_acc; p.ws_ml = ws_ml; p.ws_count = (unsigned*)ws_count;
-    p.num_pages = (int)num_pages; p.num_tokens = num_tokens; p.num_segments = num_segments;
+    p.q = (const bf16*)a.q; p.q_stride = q_stride;
+    p.kcache = (const unsigned char*)a.kcache; p.vcache = (const unsigned char*)a.vcache; p.kscale = a.kscale; p.vscale = a.vscale;
+    p.block_table = a.block_table; p.bt_rows = bt_rows; p.bt_stride = bt_stride;
+    p.seg_off = a.seg_off; p.seg_slot = a.seg_slot; p.seg_start = a.seg_start; p.seg_len = a.seg_len;
+    p.out = (bf16*)a.out; p.ws_acc = a.ws_acc; p.ws_ml = a.ws_ml; p.ws_count = (unsigned*)a.ws_count;
+    p.num_pages = (int)a.num_pages; p.num_tokens = num_tokens; p.num_segments = num_segments;
     p.nq = nq; p.nkv = nkv; p.group = nq / nkv; p.head_tiles = (p.group + A8_HEADS - 1) / A8_HEADS;
     p.window = window; p.page_shift = 0;
     while ((1 << p.page_shift) < page_size) ++p.page_shift;

@@ -343,11 +343,21 @@ static int cw_launch(const CwParams& p, int code, int* launches, cudaStream_t st
     return pi_check_launch("pi_cache_8bit_write");
 }
 
-PI_EXPORT int pi_cache_8bit_write(const void* qkv, int row_stride, const void* q_weight, const void* k_weight, int weight_dtype,
-                                  float eps, int has_norm, const float* cos_t, const float* sin_t, int rot_pairs, int adjacent,
-                                  void* kcache, void* vcache, float* kscale, float* vscale, int cache_dtype, long long num_pages,
-                                  int page_size, const long long* slot_map, void* q_out, int nq, int nkv, int head_dim,
-                                  int num_tokens, int* error_count, int* launches, cudaStream_t stream) {
+// arguments as one record of 8-byte fields
+struct CwArgs {
+    const void* qkv; long long row_stride; const void* q_weight; const void* k_weight; long long weight_dtype, has_norm;
+    const float* cos_t; const float* sin_t; long long rot_pairs, adjacent;
+    void* kcache; void* vcache; float* kscale; float* vscale; long long cache_dtype, num_pages, page_size;
+    const long long* slot_map; void* q_out; long long nq, nkv, head_dim, num_tokens; int* error_count;
+    double eps;
+};
+
+// *launches: kernels launched
+PI_EXPORT int pi_cache_8bit_write(const CwArgs* args, int* launches, cudaStream_t stream) {
+    const CwArgs& a = *args;
+    const int row_stride = (int)a.row_stride, weight_dtype = (int)a.weight_dtype, has_norm = (int)a.has_norm, rot_pairs = (int)a.rot_pairs;
+    const int adjacent = (int)a.adjacent, cache_dtype = (int)a.cache_dtype, page_size = (int)a.page_size;
+    const int nq = (int)a.nq, nkv = (int)a.nkv, head_dim = (int)a.head_dim, num_tokens = (int)a.num_tokens;
     *launches = 0;
     if (num_tokens <= 0) return 0;
     if (head_dim != 64 && head_dim != 128) return pi_refuse("pi_cache_8bit_write: head size %d is not 64 or 128", head_dim);
@@ -359,16 +369,16 @@ PI_EXPORT int pi_cache_8bit_write(const void* qkv, int row_stride, const void* q
         return pi_refuse("pi_cache_8bit_write: %d rotated pairs must be a multiple of %d and fit the head size %d", rot_pairs, adjacent ? 4 : 8, head_dim);
     if (row_stride % 8 != 0 || row_stride < (nq + 2 * nkv) * head_dim)
         return pi_refuse("pi_cache_8bit_write: rows of %d elements must be a multiple of 8 and hold all heads", row_stride);
-    if (((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)kcache | (uintptr_t)vcache | (uintptr_t)cos_t | (uintptr_t)sin_t |
-         (has_norm ? (uintptr_t)q_weight | (uintptr_t)k_weight : 0)) & 15)
+    if (((uintptr_t)a.qkv | (uintptr_t)a.q_out | (uintptr_t)a.kcache | (uintptr_t)a.vcache | (uintptr_t)a.cos_t | (uintptr_t)a.sin_t |
+         (has_norm ? (uintptr_t)a.q_weight | (uintptr_t)a.k_weight : 0)) & 15)
         return pi_refuse("pi_cache_8bit_write: tensors must start on 16-byte boundaries");
     CwParams p;
-    p.qkv = (const bf16*)qkv; p.row_stride = row_stride; p.qw = q_weight; p.kw = k_weight; p.eps = eps; p.has_norm = has_norm;
-    p.cos_t = cos_t; p.sin_t = sin_t; p.rot_pairs = rot_pairs;
-    p.kcache = (unsigned char*)kcache; p.vcache = (unsigned char*)vcache; p.kscale = kscale; p.vscale = vscale;
-    p.slot_map = slot_map; p.num_slots = num_pages * page_size; p.page_shift = 0;
+    p.qkv = (const bf16*)a.qkv; p.row_stride = row_stride; p.qw = a.q_weight; p.kw = a.k_weight; p.eps = (float)a.eps; p.has_norm = has_norm;
+    p.cos_t = a.cos_t; p.sin_t = a.sin_t; p.rot_pairs = rot_pairs;
+    p.kcache = (unsigned char*)a.kcache; p.vcache = (unsigned char*)a.vcache; p.kscale = a.kscale; p.vscale = a.vscale;
+    p.slot_map = a.slot_map; p.num_slots = a.num_pages * page_size; p.page_shift = 0;
     while ((1 << p.page_shift) < page_size) ++p.page_shift;
-    p.q_out = (bf16*)q_out; p.nq = nq; p.nkv = nkv; p.num_tokens = num_tokens; p.error_count = error_count;
+    p.q_out = (bf16*)a.q_out; p.nq = nq; p.nkv = nkv; p.num_tokens = num_tokens; p.error_count = a.error_count;
     p.kv_units = 0; p.window = p.q_shares = 1; p.wide = weight_dtype == PI_F32;
     if (adjacent)
         return head_dim == 128 ? cw_launch<128, true>(p, cache_dtype, launches, stream) : cw_launch<64, true>(p, cache_dtype, launches, stream);
@@ -472,20 +482,27 @@ __global__ void __launch_bounds__(CR_WARPS * 32) cache_8bit_read_kernel(const Cr
     }
 }
 
-PI_EXPORT int pi_cache_8bit_read(const void* kcache, const void* vcache, const float* kscale, const float* vscale, int cache_dtype,
-                                 long long num_pages, int nkv, int page_size, int head_dim, const int* page_list,
-                                 const int* page_tokens, int num_listed, void* keys, void* values, cudaStream_t stream) {
+struct CrArgs {
+    const void* kcache; const void* vcache; const float* kscale; const float* vscale;
+    long long cache_dtype, num_pages, nkv, page_size, head_dim;
+    const int* page_list; const int* page_tokens; long long num_listed; void* keys; void* values;
+};
+
+PI_EXPORT int pi_cache_8bit_read(const CrArgs* args, cudaStream_t stream) {
+    const CrArgs& a = *args;
+    const int cache_dtype = (int)a.cache_dtype, nkv = (int)a.nkv, page_size = (int)a.page_size, head_dim = (int)a.head_dim;
+    const int num_listed = (int)a.num_listed;
     if (num_listed <= 0) return 0;
     if (head_dim != 64 && head_dim != 128) return pi_refuse("pi_cache_8bit_read: head size %d is not 64 or 128", head_dim);
     if (nkv <= 0) return pi_refuse("pi_cache_8bit_read: nkv=%d", nkv);
     if (page_size < C8_BLOCK || (page_size & (page_size - 1))) return pi_refuse("pi_cache_8bit_read: page size %d must be a power of two of at least 16", page_size);
     if (cache_dtype != PI_E4M3 && cache_dtype != PI_INT8) return pi_refuse("pi_cache_8bit_read: unknown dtype code %d of the pages", cache_dtype);
-    if (((uintptr_t)kcache | (uintptr_t)vcache | (uintptr_t)keys | (uintptr_t)values) & 15)
+    if (((uintptr_t)a.kcache | (uintptr_t)a.vcache | (uintptr_t)a.keys | (uintptr_t)a.values) & 15)
         return pi_refuse("pi_cache_8bit_read: tensors must start on 16-byte boundaries");
     CrParams p;
-    p.kcache = (const unsigned char*)kcache; p.vcache = (const unsigned char*)vcache; p.kscale = kscale; p.vscale = vscale;
-    p.num_pages = num_pages; p.page_list = page_list; p.page_tokens = (const int2*)page_tokens; p.num_listed = num_listed;
-    p.keys = (bf16*)keys; p.values = (bf16*)values; p.nkv = nkv; p.page_shift = 0;
+    p.kcache = (const unsigned char*)a.kcache; p.vcache = (const unsigned char*)a.vcache; p.kscale = a.kscale; p.vscale = a.vscale;
+    p.num_pages = a.num_pages; p.page_list = a.page_list; p.page_tokens = (const int2*)a.page_tokens; p.num_listed = num_listed;
+    p.keys = (bf16*)a.keys; p.values = (bf16*)a.values; p.nkv = nkv; p.page_shift = 0;
     while ((1 << p.page_shift) < page_size) ++p.page_shift;
     const long long units = (long long)num_listed * nkv * (page_size / C8_BLOCK);
     const long long blocks = (units + CR_WARPS - 1) / CR_WARPS;

@@ -138,10 +138,19 @@ __global__ void __launch_bounds__(PM_THREADS) page_maps_kernel(const PmParams p)
     }
 }
 
-PI_EXPORT int pi_page_maps(const int* block_table, int bt_rows, int bt_stride, const int* seg_slot, const int* seg_start,
-                           const int* seg_len, int num_segments, int page_size, int num_tokens, int num_listed, int window,
-                           int min_tokens, long long* slot_map, int* positions, int* token_seg, int* seg_off, int* page_off,
-                           int* page_list, int* page_tokens, int* table, int* rows, cudaStream_t stream) {
+// arguments as one record of 8-byte fields (one pointer to pass instead of 22 values)
+struct PmArgs {
+    const int* block_table; long long bt_rows, bt_stride;
+    const int* seg_slot; const int* seg_start; const int* seg_len;
+    long long num_segments, page_size, num_tokens, num_listed, window, min_tokens;
+    long long* slot_map; int* positions; int* token_seg; int* seg_off; int* page_off; int* page_list; int* page_tokens;
+    int* table; int* rows;
+};
+
+PI_EXPORT int pi_page_maps(const PmArgs* args, cudaStream_t stream) {
+    const PmArgs& a = *args;
+    const int bt_rows = (int)a.bt_rows, bt_stride = (int)a.bt_stride, num_segments = (int)a.num_segments, page_size = (int)a.page_size;
+    const int num_tokens = (int)a.num_tokens, num_listed = (int)a.num_listed, window = (int)a.window, min_tokens = (int)a.min_tokens;
     if (num_segments <= 0) return pi_refuse("pi_page_maps: num_segments=%d must be positive", num_segments);
     if (num_segments > PM_MAX_SEGMENTS) return pi_refuse("pi_page_maps: %d segments; at most %d", num_segments, PM_MAX_SEGMENTS);
     if (page_size <= 0 || (page_size & (page_size - 1))) return pi_refuse("pi_page_maps: page_size=%d must be a power of two", page_size);
@@ -149,14 +158,14 @@ PI_EXPORT int pi_page_maps(const int* block_table, int bt_rows, int bt_stride, c
         return pi_refuse("pi_page_maps: num_tokens=%d num_listed=%d window=%d min_tokens=%d table [%d, %d]", num_tokens, num_listed,
                          window, min_tokens, bt_rows, bt_stride);
     PmParams p;
-    p.block_table = block_table; p.bt_rows = bt_rows; p.bt_stride = bt_stride;
-    p.seg_slot = seg_slot; p.seg_start = seg_start; p.seg_len = seg_len;
+    p.block_table = a.block_table; p.bt_rows = bt_rows; p.bt_stride = bt_stride;
+    p.seg_slot = a.seg_slot; p.seg_start = a.seg_start; p.seg_len = a.seg_len;
     p.num_segments = num_segments; p.num_tokens = num_tokens; p.num_listed = num_listed; p.window = window; p.min_tokens = min_tokens;
     p.page_shift = 0;
     while ((1 << p.page_shift) < page_size) ++p.page_shift;
-    p.slot_map = slot_map; p.positions = positions; p.token_seg = token_seg; p.seg_off = seg_off; p.page_off = page_off;
-    p.page_list = page_list; p.page_tokens = (int2*)page_tokens; p.table = table; p.rows = rows;
-    const long long total = (long long)num_tokens + num_listed + num_segments + 1 + (table != nullptr ? (long long)num_segments * bt_stride : 0);
+    p.slot_map = a.slot_map; p.positions = a.positions; p.token_seg = a.token_seg; p.seg_off = a.seg_off; p.page_off = a.page_off;
+    p.page_list = a.page_list; p.page_tokens = (int2*)a.page_tokens; p.table = a.table; p.rows = a.rows;
+    const long long total = (long long)num_tokens + num_listed + num_segments + 1 + (a.table != nullptr ? (long long)num_segments * bt_stride : 0);
     const long long blocks = (total + PM_PER_BLOCK - 1) / PM_PER_BLOCK;
     if (blocks > 2147483647LL) return pi_refuse("pi_page_maps: %lld entries are beyond the grid limit", total);
     const size_t smem = 2 * (size_t)(num_segments + 1) * sizeof(int);       // at most 32 KB: within the default limit

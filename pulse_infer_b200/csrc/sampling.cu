@@ -462,25 +462,35 @@ __global__ void __launch_bounds__(RULE_THREADS, 6) logit_rules_kernel(const Rule
     }
 }
 
-PI_EXPORT int pi_logit_rules(const float* logits, long long ld, float* out, long long out_ld, int rows, int vocab, const int* history,
-                             const int* history_off, int history_total, const int* prompt_len, const float* repetition,
-                             const float* frequency, const float* presence, const int* bias_off, const int* bias_tokens,
-                             const float* bias_values, int bias_total, const void* mask, int mask_rows, const int* mask_row,
-                             cudaStream_t stream) {
+// arguments as one record of 8-byte fields
+struct RuleArgs {
+    const float* logits; long long ld; float* out; long long out_ld, rows, vocab;
+    const int* history; const int* history_off; long long history_total; const int* prompt_len;
+    const float* repetition; const float* frequency; const float* presence;
+    const int* bias_off; const int* bias_tokens; const float* bias_values; long long bias_total;
+    const void* mask; long long mask_rows; const int* mask_row;
+};
+
+PI_EXPORT int pi_logit_rules(const RuleArgs* args, cudaStream_t stream) {
+    const RuleArgs& a = *args;
+    const float* logits = a.logits;
+    float* out = a.out;
+    const long long ld = a.ld, out_ld = a.out_ld, history_total = a.history_total, bias_total = a.bias_total;
+    const int rows = (int)a.rows, vocab = (int)a.vocab;
     if (rows <= 0) return 0;
     if (vocab <= 0 || ld < vocab || out_ld < vocab) return pi_refuse("pi_logit_rules: vocab=%d ld=%lld out_ld=%lld", vocab, ld, out_ld);
     if (rows > 65535) return pi_refuse("pi_logit_rules: %d rows are beyond the grid limit", rows);
     if (vocab > 2147483647 - RULE_SLICE) return pi_refuse("pi_logit_rules: vocab=%d is beyond the limit", vocab);
-    if (history_total > (1 << 30) || bias_total > (1 << 30)) return pi_refuse("pi_logit_rules: histories of %d or %d biases are beyond the limit", history_total, bias_total);
+    if (history_total > (1 << 30) || bias_total > (1 << 30)) return pi_refuse("pi_logit_rules: histories of %lld or %lld biases are beyond the limit", history_total, bias_total);
     RuleParams p;
     p.logits = logits; p.ld = ld; p.out = out; p.out_ld = out_ld; p.vocab = vocab;
     p.vec = (ld % 4 == 0 && out_ld % 4 == 0 && (((uintptr_t)logits | (uintptr_t)out) & 15) == 0) ? 1 : 0;
-    p.history = history; p.history_off = history_off; p.history_total = history_total; p.prompt_len = prompt_len;
-    p.repetition = repetition; p.frequency = frequency; p.presence = presence;
-    p.bias_off = bias_off; p.bias_tokens = bias_tokens; p.bias_values = bias_values; p.bias_total = bias_total;
-    p.mask = (const unsigned*)mask; p.mask_rows = mask_rows; p.mask_words = (vocab + 31) / 32; p.mask_row = mask_row;
+    p.history = a.history; p.history_off = a.history_off; p.history_total = (int)history_total; p.prompt_len = a.prompt_len;
+    p.repetition = a.repetition; p.frequency = a.frequency; p.presence = a.presence;
+    p.bias_off = a.bias_off; p.bias_tokens = a.bias_tokens; p.bias_values = a.bias_values; p.bias_total = (int)bias_total;
+    p.mask = (const unsigned*)a.mask; p.mask_rows = (int)a.mask_rows; p.mask_words = (vocab + 31) / 32; p.mask_row = a.mask_row;
     const dim3 grid((vocab + RULE_SLICE - 1) / RULE_SLICE, rows), threads(RULE_THREADS);
-    if (bias_off != nullptr) pi_launch(logit_rules_kernel<true>, grid, threads, 0, stream, p);
+    if (a.bias_off != nullptr) pi_launch(logit_rules_kernel<true>, grid, threads, 0, stream, p);
     else pi_launch(logit_rules_kernel<false>, grid, threads, 0, stream, p);
     return pi_check_launch("pi_logit_rules");
 }

@@ -10,46 +10,30 @@ do not take.  The reference engine stores its cache in the activation dtype only
 """
 from __future__ import annotations
 
+import ctypes
 from typing import NamedTuple
 
 import torch
 
 from . import kernels as _k
-from .kernels import F32, BF16, DecodeWorkspace, KernelError, attention_tcgen05, choose_prompt_splits
+from .kernels import (BF16, DecodeWorkspace, KernelError, _on_current_device, _Record, attention_tcgen05,
+                      choose_prompt_splits)
 
 BLOCK_TOKENS = 16
 E4M3, INT8 = 2, 3
 CACHE_8BIT_DTYPES = {torch.float8_e4m3fn: E4M3, torch.int8: INT8}
 PAGE_SIZES_8BIT = (16, 32, 64, 128)
 PAGE_MAPS_MAX_SEGMENTS = 4096
-_P, _I, _L, _F = _k.c_void_p, _k.c_int, _k.ctypes.c_longlong, _k.c_float
+_PAGE_MAPS = _Record("page_maps", "pi_page_maps", 21)
+_WRITE = _Record("cache_8bit", "pi_cache_8bit_write", 24, 1, (ctypes.c_void_p,))
+_READ = _Record("cache_8bit", "pi_cache_8bit_read", 14)
+_DECODE = _Record("attention_8bit", "pi_attention_decode_8bit", 29, 1)
 
 
-def _bound(library: str, name: str, argtypes: tuple):
-    """(library, C function) with its argument types declared: ctypes then converts plain Python numbers by itself."""
-    lib = _k._lib(library)
-    fn = getattr(lib, name)
-    if fn.argtypes is None:
-        fn.argtypes = argtypes
-    return lib, fn
-
-
-def _same_device(*tensors) -> None:
-    """All on the current CUDA device: the kernel goes to that device's current stream."""
-    for t in tensors:
-        if t is not None and not t.is_cuda:
-            raise KernelError("the kernels run on a CUDA device only; got a tensor on " + str(t.device))
-    here = torch.cuda.current_device()
-    for t in tensors:
-        if t is not None and t.get_device() != here:
-            raise KernelError(f"tensors must be on the current device cuda:{here}; got one on {t.device}")
-
-
-def _ints(dtype: torch.dtype, shape, **tensors) -> None:
-    for name, t in tensors.items():
-        if t.dtype != dtype or not t.is_contiguous() or (shape is not None and tuple(t.shape) != shape):
-            raise KernelError(f"'{name}' must be contiguous {dtype}{'' if shape is None else ' of shape ' + str(shape)}, "
-                              f"got {t.dtype} {tuple(t.shape)}")
+def _vector(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple | None = None) -> None:
+    if t.dtype is not dtype or not t.is_contiguous() or (shape is not None and t.shape != shape):
+        raise KernelError(f"'{name}' must be contiguous {dtype}{'' if shape is None else ' of shape ' + str(shape)}, got "
+                          f"{t.dtype} {tuple(t.shape)}")
 
 
 def cache_8bit_usable(head_dim: int, page_size: int) -> bool:
@@ -70,19 +54,22 @@ def cache_8bit_pools(num_pages: int, num_kv_heads: int, page_size: int, head_dim
 def _check_pools(kcache, vcache, kscale, vscale, head_dim: int | None = None, nkv: int | None = None) -> tuple:
     """(dtype code, pages, kv heads, page size, head size)"""
     code = CACHE_8BIT_DTYPES.get(kcache.dtype)
-    if code is None or vcache.dtype != kcache.dtype:
+    if code is None or vcache.dtype is not kcache.dtype:
         raise KernelError(f"8-bit pages are float8_e4m3fn or int8, keys and values alike; got {kcache.dtype} and {vcache.dtype}")
-    if kcache.dim() != 4:
-        raise KernelError(f"key pages must be [pages, kv heads, page size, d], got {tuple(kcache.shape)}")
-    pages, heads, page_size, d = kcache.shape
-    if not cache_8bit_usable(d, page_size):
+    shape = kcache.shape
+    if len(shape) != 4:
+        raise KernelError(f"key pages must be [pages, kv heads, page size, d], got {tuple(shape)}")
+    pages, heads, page_size, d = shape
+    if d not in (64, 128) or page_size not in PAGE_SIZES_8BIT:
         raise KernelError(f"8-bit pages take head sizes 64 and 128 and page sizes {PAGE_SIZES_8BIT}, not {d} and {page_size}")
     blocks = page_size // BLOCK_TOKENS
-    if tuple(vcache.shape) != (pages, heads, blocks, d, BLOCK_TOKENS):
+    if vcache.shape != (pages, heads, blocks, d, BLOCK_TOKENS):
         raise KernelError(f"value pages must be [{pages}, {heads}, {blocks}, {d}, {BLOCK_TOKENS}], got {tuple(vcache.shape)}")
-    for t in (kscale, vscale):
-        if t.dtype != torch.float32 or tuple(t.shape) != (pages, heads, blocks) or not t.is_contiguous():
-            raise KernelError(f"scales must be contiguous float32 [{pages}, {heads}, {blocks}], got {t.dtype} {tuple(t.shape)}")
+    scale_shape = (pages, heads, blocks)
+    if (kscale.shape != scale_shape or vscale.shape != scale_shape or kscale.dtype is not torch.float32
+            or vscale.dtype is not torch.float32 or not kscale.is_contiguous() or not vscale.is_contiguous()):
+        raise KernelError(f"scales must be contiguous float32 {list(scale_shape)}, got {kscale.dtype} {tuple(kscale.shape)} and "
+                          f"{vscale.dtype} {tuple(vscale.shape)}")
     if not kcache.is_contiguous() or not vcache.is_contiguous():
         raise KernelError("8-bit pages must be contiguous")
     if (head_dim is not None and head_dim != d) or (nkv is not None and nkv != heads):
@@ -113,10 +100,11 @@ def page_maps(block_table: torch.Tensor, seg_slot: torch.Tensor, seg_start: torc
     (entries behind are -1), or less (what does not fit is left out).  Segments of at least ``min_tokens`` tokens list the
     pages that their queries see, from the window's first on.  ``page_size``: a power of two.  ``with_table`` False: no
     ``table`` (None), for a step that lists nothing."""
-    _same_device(block_table, seg_slot, seg_start, seg_len)
+    device = _on_current_device((block_table, seg_slot, seg_start, seg_len))
     R = seg_slot.numel()
-    _ints(torch.int32, (R,), seg_slot=seg_slot, seg_start=seg_start, seg_len=seg_len)
-    _ints(torch.int32, None, block_table=block_table)
+    for name, t in (("seg_slot", seg_slot), ("seg_start", seg_start), ("seg_len", seg_len)):
+        _vector(name, t, torch.int32, (R,))
+    _vector("block_table", block_table, torch.int32)
     if block_table.dim() != 2 or not 1 <= R <= PAGE_MAPS_MAX_SEGMENTS:
         raise KernelError(f"page_maps takes a block table [slots, pages] and 1 to {PAGE_MAPS_MAX_SEGMENTS} segments, got "
                           f"{tuple(block_table.shape)} and {R}")
@@ -128,19 +116,19 @@ def page_maps(block_table: torch.Tensor, seg_slot: torch.Tensor, seg_start: torc
     T, N = int(num_tokens), int(num_listed_pages)
     # one allocation for all of them, the 64-bit ones first
     cells = R * W if with_table else 0
-    flat = torch.empty(4 * T + 3 * N + cells + 3 * R + 2, dtype=torch.int32, device=block_table.device)
-    slot_map, positions, token_seg, page_tokens, seg_off, page_off, page_list, table, rows = flat.split(
-        [2 * T, T, T, 2 * N, R + 1, R + 1, N, cells, R])
-    if flat.numel() >= 2147483647:
+    sizes = (2 * T, T, T, 2 * N, R + 1, R + 1, N, cells, R)
+    total = sum(sizes)
+    if total >= 2147483647:
         raise KernelError("page_maps: the maps are beyond 2^31 entries")
-    base = flat.data_ptr()
-    lib, fn = _bound("page_maps", "pi_page_maps", (_P, _I, _I, _P, _P, _P) + (_I,) * 6 + (_P,) * 10)
-    at = [0, 2 * T, 3 * T, 4 * T, 4 * T + 2 * N, 4 * T + 2 * N + R + 1, 4 * T + 2 * N + 2 * R + 2,
-          4 * T + 3 * N + 2 * R + 2, 4 * T + 3 * N + 2 * R + 2 + cells]
-    ptr = [base + 4 * a for a in at]
-    _k._check(lib, fn(block_table.data_ptr(), slots, W, seg_slot.data_ptr(), seg_start.data_ptr(), seg_len.data_ptr(), R,
-                      page_size, T, N, window or 0, min_tokens, ptr[0], ptr[1], ptr[2], ptr[4], ptr[5], ptr[6], ptr[3],
-                      ptr[7] if with_table else None, ptr[8], _k._stream()), "page_maps")
+    flat = torch.empty(total, dtype=torch.int32, device=block_table.device)
+    at, ptr = flat.data_ptr(), []
+    for n in sizes:
+        ptr.append(at)
+        at += 4 * n
+    _PAGE_MAPS(device, (block_table.data_ptr(), slots, W, seg_slot.data_ptr(), seg_start.data_ptr(), seg_len.data_ptr(), R, page_size,
+                        T, N, window or 0, min_tokens, ptr[0], ptr[1], ptr[2], ptr[4], ptr[5], ptr[6], ptr[3],
+                        ptr[7] if with_table else 0, ptr[8]))
+    slot_map, positions, token_seg, page_tokens, seg_off, page_off, page_list, table, rows = flat.split_with_sizes(sizes)
     return PageMaps(slot_map.view(torch.int64), positions, token_seg, seg_off, page_off, page_list, page_tokens.view(N, 2),
                     table.view(R, W) if with_table else None, rows)
 
@@ -157,16 +145,16 @@ def qk_norm_rope_write_8bit(qkv: torch.Tensor, q_weight, k_weight, eps: float, c
     it has to (what is there is then encoded again).  The runs of a call must lie in distinct blocks.  NaN is stored as
     zero, infinity as the largest number.  A slot outside the pool is skipped and counted, once for each of the 2 nkv heads,
     in ``error_count``.  ``q_weight``/``k_weight`` None: no per-head norm; ``cos``/``sin`` None: no rotation."""
-    _same_device(qkv, q_weight, k_weight, cos, sin, kcache, vcache, kscale, vscale, slot_map, error_count, q_out)
+    device = _on_current_device((qkv, q_weight, k_weight, cos, sin, kcache, vcache, kscale, vscale, slot_map, error_count, q_out))
     code, pages, _, page_size, d = _check_pools(kcache, vcache, kscale, vscale, head_dim, nkv)
-    if qkv.dtype != torch.bfloat16 or qkv.dim() != 2 or qkv.shape[1] != (nq + 2 * nkv) * d or qkv.stride(1) != 1:
-        raise KernelError(f"qkv must be bfloat16 [T, {(nq + 2 * nkv) * d}] with unit stride, got {qkv.dtype} {tuple(qkv.shape)}")
+    width = (nq + 2 * nkv) * d
+    if qkv.dtype is not torch.bfloat16 or qkv.dim() != 2 or qkv.shape[1] != width or qkv.stride(1) != 1:
+        raise KernelError(f"qkv must be bfloat16 [T, {width}] with unit stride, got {qkv.dtype} {tuple(qkv.shape)}")
     T = qkv.shape[0]
-    _ints(torch.int64, (T,), slot_map=slot_map)
-    _ints(torch.int32, (1,), error_count=error_count)
+    _vector("slot_map", slot_map, torch.int64, (T,))
+    _vector("error_count", error_count, torch.int32, (1,))
     has_norm = q_weight is not None
-    if has_norm and (k_weight is None or tuple(q_weight.shape) != (d,) or tuple(k_weight.shape) != (d,)
-                     or q_weight.dtype != k_weight.dtype or not q_weight.is_contiguous() or not k_weight.is_contiguous()):
+    if has_norm and (k_weight is None or q_weight.shape != (d,) or k_weight.shape != (d,) or q_weight.dtype is not k_weight.dtype or not q_weight.is_contiguous() or not k_weight.is_contiguous()):
         raise KernelError("per-head norm weights must both be contiguous, of shape (head_dim,) and one dtype")
     if (cos is None) != (sin is None):
         raise KernelError("give both rotation tables or none")
@@ -174,21 +162,19 @@ def qk_norm_rope_write_8bit(qkv: torch.Tensor, q_weight, k_weight, eps: float, c
     if cos is not None:
         rot_pairs = cos.shape[-1]
         for t in (cos, sin):
-            if t.dtype != torch.float32 or tuple(t.shape) != (T, rot_pairs) or not t.is_contiguous():
+            if t.dtype is not torch.float32 or t.shape != (T, rot_pairs) or not t.is_contiguous():
                 raise KernelError("rotation tables must be contiguous float32 [T, pairs]")
     if q_out is None:
         q_out = torch.empty((T, nq * d), dtype=torch.bfloat16, device=qkv.device)
     elif q_out.dtype != torch.bfloat16 or tuple(q_out.shape) != (T, nq * d) or not q_out.is_contiguous():
         raise KernelError(f"q_out must be contiguous bfloat16 [{T}, {nq * d}]")
-    lib, fn = _bound("cache_8bit", "pi_cache_8bit_write",
-                     (_P, _I, _P, _P, _I, _F, _I, _P, _P, _I, _I, _P, _P, _P, _P, _I, _L, _I, _P, _P, _I, _I, _I, _I, _P, _P, _P))
-    launched = _I(0)
-    _k._check(lib, fn(qkv.data_ptr(), qkv.stride(0) if T > 1 else qkv.shape[1], q_weight.data_ptr() if has_norm else None,
-                      k_weight.data_ptr() if has_norm else None, _k._code(q_weight.dtype) if has_norm else BF16, eps,
-                      1 if has_norm else 0, cos.data_ptr() if rot_pairs else None, sin.data_ptr() if rot_pairs else None,
-                      rot_pairs, 1 if adjacent_pairs else 0, kcache.data_ptr(), vcache.data_ptr(), kscale.data_ptr(),
-                      vscale.data_ptr(), code, pages, page_size, slot_map.data_ptr(), q_out.data_ptr(), nq, nkv, d, T,
-                      error_count.data_ptr(), _k.ctypes.byref(launched), _k._stream()), "qk_norm_rope_write_8bit", launches=0)
+    launched = ctypes.c_int(0)
+    _WRITE(device, (qkv.data_ptr(), qkv.stride(0) if T > 1 else width, q_weight.data_ptr() if has_norm else 0,
+                    k_weight.data_ptr() if has_norm else 0, _k._code(q_weight.dtype) if has_norm else BF16, 1 if has_norm else 0,
+                    cos.data_ptr() if rot_pairs else 0, sin.data_ptr() if rot_pairs else 0, rot_pairs, 1 if adjacent_pairs else 0,
+                    kcache.data_ptr(), vcache.data_ptr(), kscale.data_ptr(), vscale.data_ptr(), code, pages, page_size,
+                    slot_map.data_ptr(), q_out.data_ptr(), nq, nkv, d, T, error_count.data_ptr(), eps),
+           extra=(ctypes.byref(launched),), launches=0)
     _k.count_launches(launched.value)
     return q_out
 
@@ -199,12 +185,12 @@ def pages_8bit_to_bf16(kcache: torch.Tensor, vcache: torch.Tensor, kscale: torch
     """The pages ``page_list`` (int32 [N]) as bfloat16 keys and values [N, kv heads, page size, d], exactly.  Tokens outside
     ``page_tokens`` (int32 [N, 2], [first, end) per page) and pages outside the pool become zeros.  ``keys`` / ``values``:
     where to, if given (at least N pages; pages behind are left as they are)."""
-    _same_device(kcache, vcache, kscale, vscale, page_list, page_tokens, keys, values)
+    device = _on_current_device((kcache, vcache, kscale, vscale, page_list, page_tokens, keys, values))
     code, pages, nkv, page_size, d = _check_pools(kcache, vcache, kscale, vscale)
     N = page_list.numel()
-    _ints(torch.int32, (N,), page_list=page_list)
+    _vector("page_list", page_list, torch.int32, (N,))
     if page_tokens is not None:
-        _ints(torch.int32, (N, 2), page_tokens=page_tokens)
+        _vector("page_tokens", page_tokens, torch.int32, (N, 2))
     out = []
     for name, t in (("keys", keys), ("values", values)):
         if t is None:
@@ -212,10 +198,9 @@ def pages_8bit_to_bf16(kcache: torch.Tensor, vcache: torch.Tensor, kscale: torch
         elif t.dtype != torch.bfloat16 or t.dim() != 4 or t.shape[0] < N or tuple(t.shape[1:]) != (nkv, page_size, d) or not t.is_contiguous():
             raise KernelError(f"{name} must be contiguous bfloat16 [at least {N}, {nkv}, {page_size}, {d}]")
         out.append(t)
-    lib, fn = _bound("cache_8bit", "pi_cache_8bit_read", (_P, _P, _P, _P, _I, _L, _I, _I, _I, _P, _P, _I, _P, _P, _P))
-    _k._check(lib, fn(kcache.data_ptr(), vcache.data_ptr(), kscale.data_ptr(), vscale.data_ptr(), code, pages, nkv, page_size, d,
-                      page_list.data_ptr(), None if page_tokens is None else page_tokens.data_ptr(), N, out[0].data_ptr(),
-                      out[1].data_ptr(), _k._stream()), "pages_8bit_to_bf16", launches=1 if N else 0)
+    _READ(device, (kcache.data_ptr(), vcache.data_ptr(), kscale.data_ptr(), vscale.data_ptr(), code, pages, nkv, page_size, d,
+                   page_list.data_ptr(), 0 if page_tokens is None else page_tokens.data_ptr(), N, out[0].data_ptr(),
+                   out[1].data_ptr()), launches=1 if N else 0)
     return out[0], out[1]
 
 
@@ -225,19 +210,21 @@ DECODE_8BIT_PAIR_COST = 2     # units that a (request, kv head, eight query head
 
 
 def _check_queries(what, q, q_stride, num_tokens, nq, nkv, d, window, scale, out) -> torch.Tensor:
-    if q.dtype != torch.bfloat16 or q.stride(-1) != 1:
-        raise KernelError(f"{what} takes bfloat16 queries with unit stride, got {q.dtype}")
+    if q.dtype is not torch.bfloat16 or q.dim() != 2 or q.stride(1) != 1:
+        raise KernelError(f"{what} takes bfloat16 queries [tokens, width] with unit stride, got {q.dtype} {tuple(q.shape)}")
     if nq <= 0 or nkv <= 0 or nq % nkv:
         raise KernelError(f"{what}: nq={nq} must be a positive multiple of nkv={nkv}")
-    if q_stride < nq * d or q_stride % 8:
-        raise KernelError(f"{what}: a query stride of {q_stride} cannot hold {nq} heads of {d} (and must be a multiple of 8)")
-    if num_tokens < 0 or (num_tokens and (num_tokens - 1) * q_stride + nq * d > q.untyped_storage().nbytes() // 2 - q.storage_offset()):
-        raise KernelError(f"{what}: the queries do not hold {num_tokens} rows of stride {q_stride}")
+    rows, width = q.shape
+    if width < nq * d or q_stride % 8 or (rows > 1 and q_stride != q.stride(0)) or q_stride < nq * d:
+        raise KernelError(f"{what}: a query stride of {q_stride} for rows of {width} elements, {q.stride(0)} apart, with {nq} heads of "
+                          f"{d} (it must be a multiple of 8)")
+    if not 0 <= num_tokens <= rows:
+        raise KernelError(f"{what}: {num_tokens} tokens in {rows} rows of queries")
     if not scale > 0.0 or (window is not None and window <= 0):
         raise KernelError(f"{what}: scale={scale} must be positive, window={window} positive or None")
     if out is None:
         return torch.empty((num_tokens, nq * d), dtype=torch.bfloat16, device=q.device)
-    if out.dtype != torch.bfloat16 or tuple(out.shape) != (num_tokens, nq * d) or not out.is_contiguous():
+    if out.dtype is not torch.bfloat16 or out.shape != (num_tokens, nq * d) or not out.is_contiguous():
         raise KernelError(f"{what}: out must be contiguous bfloat16 [{num_tokens}, {nq * d}]")
     return out
 
@@ -252,24 +239,23 @@ def attention_decode_8bit(q: torch.Tensor, q_stride: int, kcache: torch.Tensor, 
     included - are in the pages.  ``q`` holds the normalised, rotated query heads of token t at element offset t * q_stride.
     Rows of segments of several tokens in ``out`` [num_tokens, nq d] are left as they are (``attention_prompt_8bit``).
     ``workspace`` (made here when missing): what CTAs leave for one another; launches that share one must not overlap."""
-    _same_device(q, kcache, vcache, kscale, vscale, block_table, seg_off, seg_slot, seg_start, seg_len, out)
+    device = _on_current_device((q, kcache, vcache, kscale, vscale, block_table, seg_off, seg_slot, seg_start, seg_len, out))
     code, pages, _, page_size, d = _check_pools(kcache, vcache, kscale, vscale, head_dim, nkv)
     out = _check_queries("attention_decode_8bit", q, q_stride, num_tokens, nq, nkv, d, window, scale, out)
     for name, t in (("seg_off", seg_off), ("seg_slot", seg_slot), ("seg_start", seg_start), ("seg_len", seg_len)):
-        if t.dtype != torch.int32 or not t.is_contiguous() or t.numel() < num_segments:
+        if t.dtype is not torch.int32 or not t.is_contiguous() or t.numel() < num_segments:
             raise KernelError(f"'{name}' must be contiguous int32 with {num_segments} entries")
-    _ints(torch.int32, None, block_table=block_table)
+    _vector("block_table", block_table, torch.int32)
     if block_table.dim() != 2:
         raise KernelError("the block table must be [slots, pages]")
     ws = _k._decode_workspace(workspace, d, q.device)
-    lib, fn = _bound("attention_8bit", "pi_attention_decode_8bit",
-                     (_P, _I, _P, _P, _P, _P, _I, _L, _P, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P) + (_I,) * 10 + (_F, _P))
-    _k._check(lib, fn(q.data_ptr(), q_stride, kcache.data_ptr(), vcache.data_ptr(), kscale.data_ptr(), vscale.data_ptr(), code,
-                      pages, block_table.data_ptr(), block_table.shape[0], block_table.shape[1], seg_off.data_ptr(),
-                      seg_slot.data_ptr(), seg_start.data_ptr(), seg_len.data_ptr(), out.data_ptr(), ws.acc.data_ptr(),
-                      ws.ml.data_ptr(), ws.count.data_ptr(), ws.ctas, DECODE_8BIT_SPAN_MIN if span_min is None else span_min,
-                      DECODE_8BIT_PAIR_COST if pair_cost is None else pair_cost, num_tokens, num_segments, nq, nkv, d, page_size,
-                      window or 0, scale, _k._stream()), "attention_decode_8bit")
+    bt_rows, bt_stride = block_table.shape
+    _DECODE(device, (q.data_ptr(), q_stride, kcache.data_ptr(), vcache.data_ptr(), kscale.data_ptr(), vscale.data_ptr(), code, pages,
+                     block_table.data_ptr(), bt_rows, bt_stride, seg_off.data_ptr(), seg_slot.data_ptr(), seg_start.data_ptr(),
+                     seg_len.data_ptr(), out.data_ptr(), ws.acc.data_ptr(), ws.ml.data_ptr(), ws.count.data_ptr(), ws.ctas,
+                     DECODE_8BIT_SPAN_MIN if span_min is None else span_min,
+                     DECODE_8BIT_PAIR_COST if pair_cost is None else pair_cost, num_tokens, num_segments, nq, nkv, d, page_size,
+                     window or 0, scale))
     return out
 
 
@@ -283,13 +269,14 @@ def attention_prompt_8bit(q: torch.Tensor, q_stride: int, kcache: torch.Tensor, 
     runs on the copies.  ``portions``: (start, length) of the segments of more than one token, on the host.  ``keys`` /
     ``values``: bfloat16 [listed pages, kv heads, page size, d] for the copies, made here when missing; the layers of a step
     can share them.  Rows of single-token segments in ``out`` [num_tokens, nq d] are left as they are."""
-    _same_device(q, kcache, vcache, seg_start, seg_len, out, maps.table)
+    _on_current_device((q, kcache, vcache, seg_start, seg_len, out, maps.table))
     _, _, _, page_size, d = _check_pools(kcache, vcache, kscale, vscale, head_dim, nkv)
     if maps.table is None:
         raise KernelError("attention_prompt_8bit needs page maps with their table")
     out = _check_queries("attention_prompt_8bit", q, q_stride, num_tokens, nq, nkv, d, window, scale, out)
     R = maps.rows.numel()
-    _ints(torch.int32, (R,), seg_start=seg_start, seg_len=seg_len)
+    _vector("seg_start", seg_start, torch.int32, (R,))
+    _vector("seg_len", seg_len, torch.int32, (R,))
     longest = max((n for _, n in portions), default=0)
     if longest < 2:
         return out
@@ -314,6 +301,6 @@ def attention_8bit_status() -> int:
     lib = _k._LIBS.get(("attention_8bit", None))
     if lib is None:
         return 0
-    status = _k.ctypes.c_uint(0)
-    _k._check(lib, lib.pi_attention_8bit_status(_k.ctypes.byref(status)), "attention_8bit_status", launches=0)
+    status = ctypes.c_uint(0)
+    _k._check(lib, lib.pi_attention_8bit_status(ctypes.byref(status)), "attention_8bit_status", launches=0)
     return int(status.value)

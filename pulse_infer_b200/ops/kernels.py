@@ -12,7 +12,8 @@ from __future__ import annotations
 import ctypes
 import math
 import os
-from ctypes import c_float, c_int, c_void_p
+import struct
+from ctypes import c_char_p, c_float, c_int, c_void_p
 
 import torch
 
@@ -73,8 +74,45 @@ def _prefetch_args(t: torch.Tensor | None):
     return c_void_p(t.data_ptr()), ctypes.c_ulonglong(t.numel() * t.element_size())
 
 
+# torch's current stream as a plain number.  torch.cuda.current_stream() makes a Stream object, 3 to 4 us a call - as much as
+# the launch; the binding beneath it is used where torch has it.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream() -> c_void_p:
-    return c_void_p(torch.cuda.current_stream().cuda_stream)
+    if _raw_stream is None:
+        return c_void_p(torch.cuda.current_stream().cuda_stream)
+    return c_void_p(_raw_stream(torch.cuda.current_device()))
+
+
+def _on_current_device(tensors) -> int:
+    """The current CUDA device, after checking that all tensors (None: skipped) live there."""
+    for t in tensors:
+        if t is not None and not t.is_cuda:
+            raise KernelError("the kernels run on a CUDA device only; got a tensor on " + str(t.device))
+    here = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != here:
+            raise KernelError(f"tensors must be on the current device cuda:{here}; got one on {t.device}")
+    return here
+
+
+class _Record:
+    """A launcher that takes its arguments as one record of 8-byte fields (``fields`` integers or pointers, then ``doubles``
+    floating-point numbers): packing and one pointer take a third of the time of handing 20 to 30 values to ctypes."""
+
+    def __init__(self, library: str, name: str, fields: int, doubles: int = 0, extra: tuple = ()):
+        self.library, self.name = library, name
+        self.pack = struct.Struct(f"={fields}q{doubles}d").pack
+        self.argtypes = (c_char_p,) + extra + (c_void_p,)
+
+    def __call__(self, device: int, args: tuple, extra: tuple = (), launches: int = 1) -> None:
+        lib = _LIBS.get((self.library, None)) or _lib(self.library)
+        fn = getattr(lib, self.name)
+        if fn.argtypes is None:
+            fn.argtypes = self.argtypes
+        stream = _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
+        _check(lib, fn(self.pack(*args), *extra, stream), self.name, launches)
 
 
 def _need_cuda(*tensors) -> None:
@@ -804,7 +842,7 @@ def logit_edit(logits: torch.Tensor, rows: torch.Tensor, tokens: torch.Tensor, v
                                   _p(values), c_int(n), c_int(1 if set_value else 0), _stream()), "logit_edit")
 
 
-_LOGIT_RULES = None      # (library, C function) once its argument types are declared
+_LOGIT_RULES = _Record("sampling", "pi_logit_rules", 20)
 
 
 def logit_rules(logits: torch.Tensor, history: torch.Tensor, history_off: torch.Tensor, prompt_len: torch.Tensor,
@@ -818,14 +856,8 @@ def logit_rules(logits: torch.Tensor, history: torch.Tensor, history_off: torch.
     ``bias_tokens[bias_off[r]:bias_off[r + 1]]`` are added (the last of several for one token counts); tokens whose bit is
     zero in row ``mask_row[r]`` of ``mask`` (int32 [m, ceil(V / 32)], bit v % 32 of word v / 32; row -1, or one that is not
     there: all allowed) become -inf.  ids outside the vocabulary are passed over.  ``out`` may be ``logits`` itself."""
-    global _LOGIT_RULES
-    tensors = (logits, history, history_off, prompt_len, repetition, frequency, presence, bias_off, bias_tokens, bias_values,
-               mask, mask_row, out)
-    _need_cuda(*tensors)
-    here = torch.cuda.current_device()
-    for t in tensors:
-        if t is not None and t.get_device() != here:
-            raise KernelError(f"tensors must be on the current device cuda:{here}; got one on {t.device}")
+    device = _on_current_device((logits, history, history_off, prompt_len, repetition, frequency, presence, bias_off, bias_tokens,
+                                 bias_values, mask, mask_row, out))
     if logits.dtype != torch.float32 or logits.dim() != 2 or logits.stride(1) != 1:
         raise KernelError("logits must be float32 [rows, vocabulary] with unit stride")
     n, V = logits.shape
@@ -847,16 +879,10 @@ def logit_rules(logits: torch.Tensor, history: torch.Tensor, history_off: torch.
         out = torch.empty((n, V), dtype=torch.float32, device=logits.device)
     elif out.dtype != torch.float32 or tuple(out.shape) != (n, V) or out.stride(1) != 1:
         raise KernelError(f"logit_rules: out must be float32 [{n}, {V}] with unit stride")
-    if _LOGIT_RULES is None:
-        lib = _lib("sampling")
-        P, L = c_void_p, ctypes.c_longlong
-        lib.pi_logit_rules.argtypes = [P, L, P, L, c_int, c_int, P, P, c_int, P, P, P, P, P, P, P, c_int, P, c_int, P, P]
-        _LOGIT_RULES = (lib, lib.pi_logit_rules)
-    lib, fn = _LOGIT_RULES
-    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    _check(lib, fn(logits.data_ptr(), max(logits.stride(0), V), out.data_ptr(), max(out.stride(0), V), n, V, history.data_ptr(),
-                   history_off.data_ptr(), history.numel(), prompt_len.data_ptr(), repetition.data_ptr(), frequency.data_ptr(),
-                   presence.data_ptr(), ptr(bias_off), ptr(bias_tokens), ptr(bias_values),
-                   0 if bias_tokens is None else bias_tokens.numel(), ptr(mask), 0 if mask is None else mask.shape[0],
-                   ptr(mask_row), _stream()), "logit_rules")
+    ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+    _LOGIT_RULES(device, (logits.data_ptr(), max(logits.stride(0), V), out.data_ptr(), max(out.stride(0), V), n, V, history.data_ptr(),
+                          history_off.data_ptr(), history.numel(), prompt_len.data_ptr(), repetition.data_ptr(), frequency.data_ptr(),
+                          presence.data_ptr(), ptr(bias_off), ptr(bias_tokens), ptr(bias_values),
+                          0 if bias_tokens is None else bias_tokens.numel(), ptr(mask), 0 if mask is None else mask.shape[0],
+                          ptr(mask_row)))
     return out
