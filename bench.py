@@ -238,12 +238,13 @@ def timed_prefill(engine, rng, repeats: int = 3, prompt: int | None = None, cach
     return statistics.median(times)
 
 
-def make_engine(cfg, max_batch: int, graphs: bool = True, context: int | None = None, prompt: int | None = None):
+def make_engine(cfg, max_batch: int, graphs: bool = True, context: int | None = None, prompt: int | None = None,
+                cache_dtype: str | None = None):
     from pulse_infer_b200 import Engine
     context, prompt = context or CONTEXT, prompt or PROMPT
     return Engine(None, config=cfg, seed=0, dtype="bfloat16", page_size=PAGE, max_tokens=max_batch * (context + 256),
                   max_batch_size=max_batch, chunk_size=prompt, max_tokens_per_step=prompt + max_batch,
-                  max_tokens_per_request=context + 256, use_cuda_graphs=graphs)
+                  max_tokens_per_request=context + 256, use_cuda_graphs=graphs, cache_dtype=cache_dtype)
 
 
 def run_part(args) -> dict:
@@ -256,17 +257,18 @@ def run_part(args) -> dict:
     rng = np.random.RandomState(0)
     if args.only == "prefill":
         T = args.prompt_len or PROMPT
-        engine = make_engine(cfg, args.batch, graphs=not args.no_graphs, context=max(CONTEXT, T + args.cached), prompt=max(T, 2048))
+        engine = make_engine(cfg, args.batch, graphs=not args.no_graphs, context=max(CONTEXT, T + args.cached), prompt=max(T, 2048),
+                             cache_dtype=args.cache_dtype)
         ms = timed_prefill(engine, rng, repeats=max(1, args.steps), prompt=T, cached=args.cached)
         peaks, _ = load_peaks()
         flops = prefill_flops(cfg, T) + 4.0 * cfg.num_attention_heads * cfg.head_dim * T * args.cached * cfg.num_hidden_layers
-        return {"only": "prefill", "shape": args.shape or "bench", "layers": cfg.num_hidden_layers, "tokens": T, "cached": args.cached, "ms": round(ms, 3),
+        return {"only": "prefill", "shape": args.shape or "bench", "layers": cfg.num_hidden_layers, "cache": args.cache_dtype or "bfloat16", "tokens": T, "cached": args.cached, "ms": round(ms, 3),
                 "tokens_per_s": round(T / ms * 1e3, 1), "frac": round(flops / (ms * 1e-3) / (peaks["bf16_tflops"] * 1e12), 4)}
     prompt = args.prompt_len or min(PROMPT, args.context - args.steps - args.warmup - 1)
-    engine = make_engine(cfg, args.batch, graphs=not args.no_graphs, context=args.context, prompt=prompt)
+    engine = make_engine(cfg, args.batch, graphs=not args.no_graphs, context=args.context, prompt=prompt, cache_dtype=args.cache_dtype)
     ms, launches, ctx, _, _ = timed_decode(engine, args.batch, args.steps, args.warmup, rng, False, context=args.context,
                                            prompt=prompt)
-    return {"only": "decode", "shape": args.shape or "bench", "layers": cfg.num_hidden_layers, "batch": args.batch, "context": args.context,
+    return {"only": "decode", "shape": args.shape or "bench", "layers": cfg.num_hidden_layers, "cache": args.cache_dtype or "bfloat16", "batch": args.batch, "context": args.context,
             "ms_per_step": round(ms, 4), "tokens_per_s": round(args.batch / ms * 1e3, 1), "gpu_launches": launches,
             "cuda_graphs": not args.no_graphs}
 
@@ -377,7 +379,8 @@ def run_workload(args) -> dict:
     t_build = time.time()
     engine = Engine(None, config=cfg, seed=0, dtype="bfloat16", page_size=PAGE, max_tokens=pool_tokens,
                     max_batch_size=w["max_batch"], chunk_size=args.chunk, max_tokens_per_step=args.budget,
-                    max_tokens_per_request=max(lengths) + w["new_tokens"] + PAGE, use_cuda_graphs=not args.no_graphs)
+                    max_tokens_per_request=max(lengths) + w["new_tokens"] + PAGE, use_cuda_graphs=not args.no_graphs,
+                    cache_dtype=args.cache_dtype)
     build_s = time.time() - t_build
     # warm-up: one short request end to end (library start-up, first recordings), not timed
     wid = engine.add_request(prompts[0][:64], 4, ignore_eos=True)
@@ -521,6 +524,8 @@ def main() -> int:
     ap.add_argument("--context", type=int, default=CONTEXT, help="with --only decode: the context the timed steps end at")
     ap.add_argument("--prompt-len", type=int, default=None, help="with --only: tokens of each prompt (default 2048)")
     ap.add_argument("--cached", type=int, default=0, help="with --only prefill: tokens of the request already in the cache")
+    ap.add_argument("--cache-dtype", choices=["float8_e4m3fn", "int8"], default=None,
+                    help="with --only or --workload: keep keys and values in 8 bits")
     ap.add_argument("--no-graphs", action="store_true", help="with --only: launch decode steps eagerly")
     ap.add_argument("--shape", choices=sorted(WORKLOADS), default=None,
                     help="with --only: the layer sizes of that workload's model instead of the Qwen3-8B shape")

@@ -291,15 +291,20 @@ __global__ void __launch_bounds__(A8_THREADS, 1) attn_decode_8bit_kernel(const A
     A8Piece a, b;                                         // the piece whose tiles are being asked for, and the one behind it
     a8_begin(p, meta, cta_from + of_warps.from(warp), cta_from + of_warps.from(warp + 1), ahead);
     A8Cursor cur = ahead;
-    bool asking = a8_next(p, meta, ahead, a), more = asking && a8_next(p, meta, ahead, b);
+    bool asking = a8_next(p, meta, ahead, a), more = false;
     int a_first = 0, a_done = 0, a_count = 0;             // first tile of the current batch, tiles of the piece asked for
     int a_ids = -1, a_ids_next = -1, b_ids = -1;
     if (asking) {
         a_first = a.tile;
         a_ids = lookup(a, a.tile);
         a_ids_next = a.ntiles > 8 ? lookup(a, a.tile + 8) : -1;
-        if (more) b_ids = lookup(b, b.tile);
     }
+    auto look_behind = [&]() {                            // the piece behind a
+        more = asking && a8_next(p, meta, ahead, b);
+        if (more) b_ids = lookup(b, b.tile);
+    };
+    const bool short_first = asking && a.ntiles < (RING + 3) / 4;      // else the first units are all a's: they go first
+    if (short_first) look_behind();
     const unsigned ring = (unsigned)__cvta_generic_to_shared(sh.ring[warp]);
     int put = 0, take = 0, phase = 0;                     // units to fill and to use next, parity of the latter
     int pending = 0;                                      // units asked for and not used yet
@@ -336,11 +341,8 @@ __global__ void __launch_bounds__(A8_THREADS, 1) attn_decode_8bit_kernel(const A
                     a = b; a_done = 0; a_first = b.tile;
                     a_ids = b_ids;
                     asking = more;
-                    if (asking) {
-                        a_ids_next = a.ntiles > 8 ? lookup(a, a.tile + 8) : -1;
-                        more = a8_next(p, meta, ahead, b);
-                        if (more) b_ids = lookup(b, b.tile);
-                    }
+                    if (asking) a_ids_next = a.ntiles > 8 ? lookup(a, a.tile + 8) : -1;
+                    look_behind();
                 } else if ((a_done & 7) == 0) {
                     a_first += 8;
                     a_ids = a_ids_next;
@@ -365,6 +367,7 @@ __global__ void __launch_bounds__(A8_THREADS, 1) attn_decode_8bit_kernel(const A
     };
 #pragma unroll
     for (int u = 0; u < RING; ++u) ask(u & 3);
+    if (!short_first) look_behind();
 
     int count = 0;
     A8Piece w;
@@ -580,7 +583,8 @@ __global__ void __launch_bounds__(A8_THREADS, 1) attn_decode_8bit_kernel(const A
             }
         }
     }
-    pdl_trigger();                         // all keys and values are in: the next kernel may take the memory system
+    // (The next kernel is not let in early: with a pdl_trigger() here the product behind this
+    // kernel spreads unevenly over the SMs that end first, and a decode step of 36 layers goes from 3.9 to 6.3 ms.)
     __syncthreads();
     // ---- triples that were cut between the warps of the CTA: their parts are added up in warp order.  Join 0 is a triple that
     // began before the CTA, at most one of the others goes on behind it; these two leave their sum in the workspace -----------

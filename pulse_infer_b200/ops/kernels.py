@@ -77,6 +77,7 @@ def _prefetch_args(t: torch.Tensor | None):
 # torch's current stream as a plain number.  torch.cuda.current_stream() makes a Stream object, 3 to 4 us a call - as much as
 # the launch; the binding beneath it is used where torch has it.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_raw_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)      # the same for the current device
 
 
 def _stream() -> c_void_p:
@@ -87,12 +88,10 @@ def _stream() -> c_void_p:
 
 def _on_current_device(tensors) -> int:
     """The current CUDA device, after checking that all tensors (None: skipped) live there."""
+    here = _raw_device() if tensors[0].is_cuda else -1
     for t in tensors:
-        if t is not None and not t.is_cuda:
-            raise KernelError("the kernels run on a CUDA device only; got a tensor on " + str(t.device))
-    here = torch.cuda.current_device()
-    for t in tensors:
-        if t is not None and t.get_device() != here:
+        if t is not None and (t.get_device() != here or here < 0):
+            _need_cuda(t)
             raise KernelError(f"tensors must be on the current device cuda:{here}; got one on {t.device}")
     return here
 
