@@ -676,14 +676,16 @@ __global__ void __launch_bounds__(A8_THREADS, 1) attn_decode_8bit_kernel(const A
 template <int D, bool E4M3>
 static int a8_launch(const A8Params& p, int ctas, cudaStream_t stream) {
     const size_t smem = sizeof(A8Shared<D>);
-    static bool configured = false;
-    if (!configured) {
+    static bool configured[64] = {};                          // per device: the attribute belongs to a device's copy of the kernel
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return pi_refuse("pi_attention_decode_8bit: no current device below 64");
+    if (!configured[device]) {
         cudaError_t err = cudaFuncSetAttribute(attn_decode_8bit_kernel<D, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (err != cudaSuccess) {
             snprintf(g_pi_error, sizeof(g_pi_error), "pi_attention_decode_8bit: cannot reserve %zu bytes of shared memory: %s", smem, cudaGetErrorString(err));
             return (int)err;
         }
-        configured = true;
+        configured[device] = true;
     }
     pi_launch(attn_decode_8bit_kernel<D, E4M3>, dim3((unsigned)ctas), dim3(A8_THREADS), smem, stream, p);
     return pi_check_launch("pi_attention_decode_8bit");

@@ -860,6 +860,8 @@ def logit_rules(logits: torch.Tensor, history: torch.Tensor, history_off: torch.
     if logits.dtype != torch.float32 or logits.dim() != 2 or logits.stride(1) != 1:
         raise KernelError("logits must be float32 [rows, vocabulary] with unit stride")
     n, V = logits.shape
+    if n > 1 and logits.stride(0) < V:
+        raise KernelError("logit_rules: the rows of the logits overlap")
     for name, t, dtype, size in (("history", history, torch.int32, None), ("history_off", history_off, torch.int32, n + 1),
                                  ("prompt_len", prompt_len, torch.int32, n), ("repetition", repetition, torch.float32, n),
                                  ("frequency", frequency, torch.float32, n), ("presence", presence, torch.float32, n)):
@@ -876,10 +878,11 @@ def logit_rules(logits: torch.Tensor, history: torch.Tensor, history_off: torch.
         raise KernelError(f"logit_rules: mask must be contiguous int32 [rows, {(V + 31) // 32}], mask_row int32 [{n}]")
     if out is None:
         out = torch.empty((n, V), dtype=torch.float32, device=logits.device)
-    elif out.dtype != torch.float32 or tuple(out.shape) != (n, V) or out.stride(1) != 1:
-        raise KernelError(f"logit_rules: out must be float32 [{n}, {V}] with unit stride")
+    elif out.dtype != torch.float32 or tuple(out.shape) != (n, V) or out.stride(1) != 1 or (n > 1 and out.stride(0) < V):
+        raise KernelError(f"logit_rules: out must be float32 [{n}, {V}] with unit stride and rows apart")
     ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
-    _LOGIT_RULES(device, (logits.data_ptr(), max(logits.stride(0), V), out.data_ptr(), max(out.stride(0), V), n, V, history.data_ptr(),
+    ld, out_ld = (logits.stride(0), out.stride(0)) if n > 1 else (V, V)
+    _LOGIT_RULES(device, (logits.data_ptr(), ld, out.data_ptr(), out_ld, n, V, history.data_ptr(),
                           history_off.data_ptr(), history.numel(), prompt_len.data_ptr(), repetition.data_ptr(), frequency.data_ptr(),
                           presence.data_ptr(), ptr(bias_off), ptr(bias_tokens), ptr(bias_values),
                           0 if bias_tokens is None else bias_tokens.numel(), ptr(mask), 0 if mask is None else mask.shape[0],

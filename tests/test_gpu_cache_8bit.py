@@ -560,3 +560,28 @@ def test_a_wait_that_runs_out_is_reported_and_the_next_launch_works(monkeypatch,
     _decode(ops, dev, torch.int8, [1600], 4, 1, 128, 16, workspace=ws)
     assert ops.attention_8bit_status() == 0
     runner.check_device_errors()
+
+
+@pytest.mark.parametrize("requests", [257, 1024])
+def test_decode_a_great_many_short_requests(requests):
+    """More requests than threads in a block, most of them a tile or two long, some of no length at all."""
+    lengths = [1 + (i * 37) % 70 for i in range(requests)]
+    lengths[5] = 900
+    _decode(_ops(), need_gpu(), torch.int8, lengths, 2, 1, 64, 16, seed=requests)
+
+
+def test_calls_without_tokens():
+    dev, ops = need_gpu(), _ops()
+    pools = ops.cache_8bit_pools(2, 2, 16, 64, torch.float8_e4m3fn, dev)
+    before = [p.clone() for p in pools]
+    err = torch.zeros(1, dtype=torch.int32, device=dev)
+    q = ops.qk_norm_rope_write_8bit(torch.empty(0, 512, dtype=torch.bfloat16, device=dev), None, None, 1e-6, None, None, True, *pools,
+                                    torch.empty(0, dtype=torch.int64, device=dev), 4, 2, 64, err)
+    assert q.shape == (0, 256) and all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(pools, before))
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+    q = torch.zeros(3, 256, dtype=torch.bfloat16, device=dev)
+    out = torch.full((3, 256), 5.0, dtype=torch.bfloat16, device=dev)
+    for start, length in (((0, 3), (0, 3)), ((-4, 0), (1, 0))):           # no segment of one token, or one at no position
+        ops.attention_decode_8bit(q, 256, *pools, torch.zeros(2, 2, dtype=torch.int32, device=dev), i32(0, 0), i32(0, 1), i32(*start),
+                                  i32(*length), 3, 2, 4, 2, 64, None, 0.1, out=out)
+        assert (out == 5).all()

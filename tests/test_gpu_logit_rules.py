@@ -218,3 +218,21 @@ def test_engine_generates_under_rules(model_folders):
     assert [t % 7 for t in out[0][:4]] == [0, 1, 2, 3] and grammar.seen == [out[0][:i] for i in range(6)]
     assert len(set(out[1])) == 12 and out[2] == [17] * 5
     assert len(out[3]) == 12
+
+
+def test_logit_rules_rows_that_overlap_are_refused_and_one_row_may_have_any_stride():
+    from pulse_infer_b200.ops import KernelError
+    dev, ops = need_gpu(), _ops()
+    V = 100
+    x, *rules = _case(2, V, 4, with_bias=False, with_mask=False)
+    args, _ = _tensors(dev, V, *rules)
+    with pytest.raises(KernelError):
+        ops.logit_rules(torch.zeros(1, V, device=dev).expand(2, V), *args)
+    with pytest.raises(KernelError):
+        ops.logit_rules(torch.zeros(2, V, device=dev), *args, out=torch.zeros(1, V, device=dev).expand(2, V))
+    one = [[r[0]] if isinstance(r, list) else r[:1] for r in rules]
+    args, _ = _tensors(dev, V, *one)
+    src = torch.tensor(x[:1], device=dev)
+    odd = torch.empty_strided((1, V), (3, 1), device=dev)
+    odd.copy_(src)
+    assert torch.equal(ops.logit_rules(odd, *args), ops.logit_rules(src, *args))
