@@ -514,36 +514,62 @@ attn_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     }
 }
 
-// Combine the shares of the keys that attn_tcgen05_kernel left for the rows of prompt portions: one block per
-// (token, head), one thread per element of the head.  out = sum_s 2^(m_s - M) acc_s / sum_s 2^(m_s - M) l_s, the shares
-// taken in order; a share that saw no key (l = 0) is skipped.
+// Combine the shares of the keys that attn_tcgen05_kernel left for the rows of prompt portions: one warp per (token, head),
+// four (head size 64: two) consecutive elements per lane.  out = sum_s 2^(m_s - M) acc_s / sum_s 2^(m_s - M) l_s, the shares
+// taken in order; a share that saw no key (l = 0) is skipped.  All loads of eight shares are in flight at once: with a thread
+// per element and one share after the other, 4,096 rows of nine shares took 13.2 us instead of 7.8.
+#define FA_MERGE_WARPS 8
 template <int D>
-__global__ void attn_prompt_merge_kernel(const float* __restrict__ part_acc, const float* __restrict__ part_ml, int splits,
+__global__ void __launch_bounds__(FA_MERGE_WARPS * 32) attn_prompt_merge_kernel(const float* __restrict__ part_acc, const float* __restrict__ part_ml, int splits,
                                          bf16* __restrict__ out, const int* __restrict__ token_seg,
-                                         const int* __restrict__ seg_len, int nq) {
+                                         const int* __restrict__ seg_len, int nq, long long rows) {
+    constexpr int E = D / 32, BATCH = 8;
+    struct alignas(4 * E) Elements { float v[E]; };
     pdl_wait();
     pdl_trigger();
-    const int row = blockIdx.x, t = row / nq;
+    const long long row = (long long)blockIdx.x * FA_MERGE_WARPS + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (row >= rows) return;
+    const int t = (int)(row / nq);
     if (seg_len[token_seg[t]] == 1) return;          // single tokens are the decode kernel's
     const float2* ml = reinterpret_cast<const float2*>(part_ml + (size_t)row * splits * 2);
-    const float* acc = part_acc + (size_t)row * splits * D;
+    const float* acc = part_acc + (size_t)row * splits * D + E * lane;
     float mstar = -INFINITY;
-    for (int s = 0; s < splits; ++s) {
-        const float2 v = ml[s];
-        if (v.y > 0.0f) mstar = fmaxf(mstar, v.x);
+    for (int s0 = 0; s0 < splits; s0 += BATCH) {
+        float2 v[BATCH];
+#pragma unroll
+        for (int s = 0; s < BATCH; ++s) v[s] = s0 + s < splits ? ml[s0 + s] : make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int s = 0; s < BATCH; ++s)
+            if (v[s].y > 0.0f) mstar = fmaxf(mstar, v[s].x);
     }
-    for (int e = threadIdx.x; e < D; e += blockDim.x) {
-        float num = 0.0f, den = 0.0f;
-        for (int s = 0; s < splits; ++s) {
-            const float2 v = ml[s];
-            if (v.y > 0.0f) {
-                const float w = fa_ex2(v.x - mstar);
-                num += w * acc[(size_t)s * D + e];
-                den += w * v.y;
+    float num[E], den = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) num[e] = 0.0f;
+    for (int s0 = 0; s0 < splits; s0 += BATCH) {
+        float2 v[BATCH];
+        Elements a[BATCH];
+#pragma unroll
+        for (int s = 0; s < BATCH; ++s) {
+            v[s] = s0 + s < splits ? ml[s0 + s] : make_float2(0.0f, 0.0f);
+            if (s0 + s < splits) a[s] = *reinterpret_cast<const Elements*>(acc + (size_t)(s0 + s) * D);
+        }
+#pragma unroll
+        for (int s = 0; s < BATCH; ++s) {
+            if (v[s].y > 0.0f) {
+                const float w = fa_ex2(v[s].x - mstar);
+#pragma unroll
+                for (int e = 0; e < E; ++e) num[e] += w * a[s].v[e];
+                den += w * v[s].y;
             }
         }
-        out[(size_t)row * D + e] = __float2bfloat16_rn(den > 0.0f ? num / den : 0.0f);
     }
+    __nv_bfloat162 o[E / 2];
+#pragma unroll
+    for (int e = 0; e < E / 2; ++e)
+        o[e] = __floats2bfloat162_rn(den > 0.0f ? num[2 * e] / den : 0.0f, den > 0.0f ? num[2 * e + 1] / den : 0.0f);
+    struct alignas(2 * E) Packed { __nv_bfloat162 v[E / 2]; };
+    *reinterpret_cast<Packed*>(out + (size_t)row * D + E * lane) = *reinterpret_cast<const Packed*>(o);
 }
 
 // =============================================================================================================
@@ -1326,6 +1352,8 @@ PI_EXPORT int pi_attention_tcgen05(const void* q, int q_stride, const void* kcac
     if (splits < 1 || splits > 64) return pi_refuse("pi_attention_tcgen05: splits=%d must be 1..64", splits);
     if (splits > 1 && (part_acc == nullptr || part_ml == nullptr || token_seg == nullptr || num_tokens <= 0))
         return pi_refuse("pi_attention_tcgen05: key splitting needs its scratch, the token-to-segment table and the token count");
+    if (splits > 1 && (((uintptr_t)part_acc & 15) || ((uintptr_t)part_ml & 7) || ((uintptr_t)out & 7)))
+        return pi_refuse("pi_attention_tcgen05: the scratch of key splitting must start on 16-byte boundaries, the output on 8-byte ones");
     if (!(scale > 0.0f)) return pi_refuse("pi_attention_tcgen05: the score scale must be positive");
     if (nq <= 0 || nkv <= 0 || nq % nkv != 0) return pi_refuse("pi_attention_tcgen05: nq=%d must be a positive multiple of nkv=%d", nq, nkv);
     if (!pi_attention_tcgen05_supported(page_size)) return pi_refuse("pi_attention_tcgen05: page size %d is not one of 8, 16, 32, 64, 128", page_size);
@@ -1362,8 +1390,9 @@ PI_EXPORT int pi_attention_tcgen05(const void* q, int q_stride, const void* kcac
     pi_launch(kernel, dim3((unsigned)ctas, (unsigned)splits), dim3(FA_THREADS), smem, stream, mk, mv, p);
     rc = pi_check_launch("pi_attention_tcgen05");
     if (rc || splits == 1) return rc;
-    pi_launch(attn_prompt_merge_kernel<PI_HEAD_DIM>, dim3((unsigned)((long long)num_tokens * nq)), dim3(PI_HEAD_DIM), 0, stream,
-              (const float*)part_acc, (const float*)part_ml, splits, (bf16*)out, token_seg, seg_len, nq);
+    const long long merge_rows = (long long)num_tokens * nq;
+    pi_launch(attn_prompt_merge_kernel<PI_HEAD_DIM>, dim3((unsigned)((merge_rows + FA_MERGE_WARPS - 1) / FA_MERGE_WARPS)), dim3(FA_MERGE_WARPS * 32), 0,
+              stream, (const float*)part_acc, (const float*)part_ml, splits, (bf16*)out, token_seg, seg_len, nq, merge_rows);
     return pi_check_launch("pi_attention_tcgen05 merge");
 }
 
