@@ -1,16 +1,16 @@
 // Decode attention over 8-bit key/value pages (format: cache_8bit.cuh): segments of one token,
 //   out = softmax(scale * q K^T) V,  K = 2^ek k8,  V = 2^ev v8,  keys lo .. pos (lo = pos - window + 1 with a window)
 //
-// All of it is memory traffic - each byte of a key or value is used for a handful of query heads.  A warp takes 64 keys (four
-// blocks of 16) at a time, in four units (two of keys, two of values, 4 KB each for D = 128), which come through a queue in
-// shared memory that belongs to it alone: bulk copies of half a block, an mbarrier per unit, no exchange between warps, and
-// 128 to 160 KB per SM in flight.  (Lanes that fetch their 16-byte operand pieces themselves, into registers or with
-// cp.async, ask for 32 or 64 bytes of a line at a time; that path delivers 4.7 and 4.0 TB/s, from L2 no more.)
+// All of it is memory traffic - each byte of a key or value is used for a handful of query heads - so keys and values go
+// straight from memory into the registers in which mma.sync wants them, in 16-byte pieces, and nothing is exchanged between
+// warps until all work is done.  A warp takes 64 keys (four blocks of 16) at a time: while it computes the scores of a tile
+// its values are on their way, and as soon as a register of keys or values has been used, the next tile's is asked for: 8 to
+// 16 KB per warp, about 100 KB per SM, in flight.
 //   S^T = K Q^T      m16n8k16, 16 keys x 8 query heads; the codes become half precision exactly (two instructions for four
 //                    e4m3, five for int8), queries are scaled to [1, 2) per head so that half precision holds them
 //   softmax          in 32 bits; a value block's scale joins the exponent: w = 2^(s + ev - m'), m' the running maximum of
 //                    s + ev, so the weights of the second product are at most 1 whatever the scales are (half precision
-//                    rounds them by 2^-12), and the sum of 2^(s - m') is kept beside it
+//                    rounds them by up to 2^-11), and the sum of 2^(s - m') is kept beside it
 //   O^T += V^T w^T   m16n8k16, 16 elements of the head x 8 query heads; movmatrix turns the weights, and V^T is what the
 //                    pages hold
 // The contractions do not care in which order keys or elements come, so the order is the one in which a lane's pieces lie:
@@ -26,24 +26,21 @@
 // CTA that delivers a triple's last missing piece adds the pieces up in the order of the keys.  Nothing waits for another CTA.
 // A group of more than eight query heads is cut in pieces of eight, and its keys are read once for each (from L2 mostly).
 //
-// Measured (B200, e4m3, 8 kv heads of 128; device time of a launch among others): 64 requests of 130 to 8,190 keys, 40 query
-// heads: 83 us, 459 MB at 5.5 TB/s (6.9 while the queues run); 8 requests of 4,096 keys: 22 us, of which 10 are transfer, 4
-// the way to the first byte (lengths, block table, copies: three round trips) and 6 the sums between warps and CTAs at the end.
-// Every wait is bounded; after one that ran out the kernel records a code and goes on without data.
+// Measured (B200, 8 kv heads of 128; device time of a launch among others): 64 requests of 130 to 8,190 keys, 40 query heads,
+// e4m3: 85 us, 459 MB at 5.4 TB/s (6.9 in the middle); 8 requests of 4,096 keys: 21.4 us, of which 10 are transfer, 3 to 4 the way
+// to the first byte (lengths, block table, pages: three round trips) and 5 the sums between warps and CTAs at the end; one of
+// 32,768 keys, int8: 23.4 us.  Tried: operands through a queue in shared memory of each warp, by bulk copies with an mbarrier per
+// 4 KB (83, 22.7 and 25.4 us; also with 12 warps) or by cp.async (slower still); spans of whole CTAs, a barrier at each piece
+// (113, 25.8 and 31.7 us).
 #include <math.h>
 
 #include "cache_8bit.cuh"
 
-// 8 warps with 5 units each (12 with 3: the same within 3 %, 10 with 4 no better)
 #define A8_WARPS 8
-#define A8_RING 5              // units of a warp's queue for D = 128, twice as many for D = 64
 #define A8_THREADS (A8_WARPS * 32)
 #define A8_TILE 64
 #define A8_HEADS 8
 #define A8_MAX_SEGS 1024
-#ifndef A8_SPIN_LIMIT
-#define A8_SPIN_LIMIT (1u << 22)
-#endif
 #define A8_SLOT_HEADS 16       // heads per slot of the workspace
 
 struct A8Params {
@@ -102,30 +99,12 @@ __device__ __forceinline__ unsigned a8_turn(unsigned x) {
     return y;
 }
 
-__device__ __forceinline__ void a8_copy4(unsigned dst, const void* src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void a8_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void a8_wait_group() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
-__device__ __forceinline__ void a8_bulk(unsigned dst, const void* src, unsigned bytes, unsigned bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
-                 "r"(bytes), "r"(bar) : "memory");
-}
-__device__ __forceinline__ void a8_expect(unsigned bar, unsigned bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-// false: the wait ran out (A8_SPIN_LIMIT polls); the status word then names the warp and the unit
-__device__ unsigned g_a8_status;
-__device__ __forceinline__ bool a8_arrived(unsigned bar, unsigned parity, unsigned code) {
-    for (unsigned i = 0; i < A8_SPIN_LIMIT; ++i) {
-        unsigned done;
-        asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
-                     : "=r"(done) : "r"(bar), "r"(parity) : "memory");
-        if (done) return true;
-    }
-    atomicCAS(&g_a8_status, 0u, code);
-    return false;
+__device__ __forceinline__ uint4 a8_load(const unsigned char* p) {
+    uint4 v;
+    // not the read-only path: the pages were written by the kernel before this one, which may still have been running when
+    // this kernel began
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
 }
 
 __device__ __forceinline__ unsigned a8_word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
@@ -189,17 +168,8 @@ struct A8Join {
 template <int D>
 struct A8Shared {
     static constexpr int LINE = D + 4;                    // floats of a head's line: no bank conflicts
-    static constexpr int HALF = 8 * D;                    // bytes of half a block: eight keys, or D / 2 lines of values
-    static constexpr int PITCH = HALF + 32;               // of the four in a unit: keeps value reads free of bank conflicts
-    static constexpr int UNIT = 4 * PITCH;
-    static constexpr int RING = A8_RING * 128 / D;        // units of the queue
-    static constexpr int TILES = 4;                       // tiles whose block numbers and scales are kept
-    alignas(16) unsigned char ring[A8_WARPS][RING * UNIT];   // the queue; afterwards the part of the triple that the warp began last
-    float part0[A8_WARPS][A8_HEADS][LINE];                // the part of the triple that began before the warp's span
+    float parts[A8_WARPS * 2][A8_HEADS][LINE];            // per warp: of the triple that began before its span, and of one that begins in it
     float m[A8_WARPS * 2][A8_HEADS], l[A8_WARPS * 2][A8_HEADS];
-    int id[A8_WARPS][TILES][4];
-    float ks[A8_WARPS][TILES][4], vs[A8_WARPS][TILES][4];
-    unsigned long long bar[A8_WARPS][RING];               // a unit has arrived
     A8Meta meta;
     int scan[32];
     A8Join join[A8_WARPS + 1];
@@ -207,10 +177,7 @@ struct A8Shared {
     int cut[2];                                           // which join left its sum in workspace slot 0 and 1; -1: none
     int last[2];
 
-    // accumulators of a part: which = 0 for a triple that began before the span of the warp, 1 for one that begins in it
-    __device__ __forceinline__ float* part(int warp, int which, int head) {
-        return which ? reinterpret_cast<float*>(ring[warp]) + head * LINE : part0[warp][head];
-    }
+    __device__ __forceinline__ float* part(int warp, int which, int head) { return parts[2 * warp + which][head]; }
 };
 
 template <int D, bool E4M3>
@@ -218,20 +185,14 @@ __global__ void __launch_bounds__(A8_THREADS, 1) attn_decode_8bit_kernel(const A
     typedef A8Shared<D> Shared;
     constexpr int KC = D / 64;             // 16-byte pieces of a key row per lane
     constexpr int KS = D / 16;             // k steps of the first product, and 16-row tiles of V^T
-    constexpr int RING = Shared::RING, UNIT = Shared::UNIT;
-    static_assert(Shared::RING * Shared::UNIT >= A8_HEADS * Shared::LINE * 4, "a part fits the queue");
     extern __shared__ __align__(16) unsigned char a8_smem[];
     Shared& sh = *reinterpret_cast<Shared*>(a8_smem);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const A8Meta& meta = sh.meta;
-    const unsigned bars = (unsigned)__cvta_generic_to_shared(sh.bar[warp]);
     if (threadIdx.x < 2) sh.cut[threadIdx.x] = -1;
     if (threadIdx.x == 0) { sh.joins = 0; sh.join[0].heads = 0; }
     if (threadIdx.x < A8_WARPS * 2 * A8_HEADS) { (&sh.m[0][0])[threadIdx.x] = -INFINITY; (&sh.l[0][0])[threadIdx.x] = 0.0f; }
     static_assert(A8_WARPS * 2 * A8_HEADS <= A8_THREADS, "one thread per entry");
-    if (lane < RING) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bars + 8 * lane) : "memory");
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     pdl_wait();
     const int page_blocks = 1 << (p.page_shift - 4);
     {   // the segments' units, summed up by the whole block
@@ -277,101 +238,45 @@ __global__ void __launch_bounds__(A8_THREADS, 1) attn_decode_8bit_kernel(const A
     const int cta_from = of_ctas.from(blockIdx.x), cta_len = of_ctas.from(blockIdx.x + 1) - cta_from;
     const A8Shares of_warps(cta_len, A8_WARPS);
 
-    // ---- the queue: units K K V V of one tile after the other, piece after piece ------------------------------------
-    // Block numbers are looked up 32 at a time (lane = block, eight tiles), one batch ahead of use, the first ones of a piece
-    // while the piece before it is asked for: a look-up is two dependent loads, and a tile must not wait for them.
-    auto lookup = [&](const A8Piece& x, int tile) -> int {     // -1: a block without visible keys or without a page
-        const int key = tile * A8_TILE + lane * C8_BLOCK;
+    // block (lane >> 3) of a tile of piece x: its number in the pool, -1 if it holds no visible key or has no page
+    auto lookup = [&](const A8Piece& x, int tile) -> int {
+        const int key = tile * A8_TILE + (lane >> 3) * C8_BLOCK;
         if (x.slot < 0 || x.slot >= p.bt_rows || key > x.pos || key + C8_BLOCK <= x.lo) return -1;
         const int page = p.block_table[(size_t)x.slot * p.bt_stride + (key >> p.page_shift)];
         if (page < 0 || page >= p.num_pages) return -1;
         return (page * p.nkv + x.kvh) * page_blocks + ((key & ((1 << p.page_shift) - 1)) >> 4);
     };
-    A8Cursor ahead;
-    A8Piece a, b;                                         // the piece whose tiles are being asked for, and the one behind it
-    a8_begin(p, meta, cta_from + of_warps.from(warp), cta_from + of_warps.from(warp + 1), ahead);
-    A8Cursor cur = ahead;
-    bool asking = a8_next(p, meta, ahead, a), more = false;
-    int a_first = 0, a_done = 0, a_count = 0;             // first tile of the current batch, tiles of the piece asked for
-    int a_ids = -1, a_ids_next = -1, b_ids = -1;
-    if (asking) {
-        a_first = a.tile;
-        a_ids = lookup(a, a.tile);
-        a_ids_next = a.ntiles > 8 ? lookup(a, a.tile + 8) : -1;
-    }
-    auto look_behind = [&]() {                            // the piece behind a
-        more = asking && a8_next(p, meta, ahead, b);
-        if (more) b_ids = lookup(b, b.tile);
-    };
-    const bool short_first = asking && a.ntiles < (RING + 3) / 4;      // else the first units are all a's: they go first
-    if (short_first) look_behind();
-    const unsigned ring = (unsigned)__cvta_generic_to_shared(sh.ring[warp]);
-    int put = 0, take = 0, phase = 0;                     // units to fill and to use next, parity of the latter
-    int pending = 0;                                      // units asked for and not used yet
-    bool ok = true;                                       // no wait has run out
-    // unit 0, 1: keys 8 unit .. + 7 of the four blocks; 2, 3: their lines (unit - 2) D / 2 .. of V^T.  Lane b < 4 copies block
-    // b; in the place of a block that is not there comes block 0, to be masked.
-    auto ask = [&](int unit) {
-        if (asking && ok) {
-            const int at4 = 4 * (a_done & 7);              // the tile's first block in the batch
-            const int id = __shfl_sync(0xffffffffu, a_ids, at4 + t);
-            if (unit == 0 && lane < 4) {
-                const int at = a_count & (Shared::TILES - 1);
-                sh.id[warp][at][lane] = id;
-                a8_copy4((unsigned)__cvta_generic_to_shared(&sh.ks[warp][at][lane]), p.kscale + max(id, 0));
-                a8_copy4((unsigned)__cvta_generic_to_shared(&sh.vs[warp][at][lane]), p.vscale + max(id, 0));
-            }
-            const unsigned bar = bars + 8 * put;
-            if (lane == 0) a8_expect(bar, 4 * Shared::HALF);
-            __syncwarp();                                  // the unit that lay here has been read by all lanes
-            ++pending;
-#ifdef A8_TEST_HOOKS
-            // test build: one copy is left out, so the wait for its unit runs out
-            const bool copies = lane < 4 && !(blockIdx.x == 0 && warp == 1 && a_count == 1 && unit == 2 && lane == 3);
-#else
-            const bool copies = lane < 4;
-#endif
-            if (copies)
-                a8_bulk(ring + put * UNIT + lane * Shared::PITCH,
-                        (unit < 2 ? p.kcache : p.vcache) + (size_t)max(id, 0) * (C8_BLOCK * D) + (unit & 1) * Shared::HALF, Shared::HALF, bar);
-            if (unit == 3) {                              // the next tile, or the next piece's first
-                ++a_count;
-                ++a_done;
-                if (a_done == a.ntiles) {
-                    a = b; a_done = 0; a_first = b.tile;
-                    a_ids = b_ids;
-                    asking = more;
-                    if (asking) a_ids_next = a.ntiles > 8 ? lookup(a, a.tile + 8) : -1;
-                    look_behind();
-                } else if ((a_done & 7) == 0) {
-                    a_first += 8;
-                    a_ids = a_ids_next;
-                    a_ids_next = a_done + 8 < a.ntiles ? lookup(a, a_first + 8) : -1;
-                }
-            }
-        }
-        if (unit == 0) a8_commit();                        // a group of scale copies per tile
-        put = put + 1 == RING ? 0 : put + 1;
-    };
-    // The next unit.  After a wait that ran out nothing more is asked for, the copies under way are still waited for (with the
-    // same limit), and the warp goes through the rest of its span without data.
-    auto arrived = [&]() {
-        if (pending > 0) {
-            const bool here = a8_arrived(bars + 8 * take, phase, 0x8b000000u | (blockIdx.x << 8) | (warp << 4) | take);
-            ok = __all_sync(0xffffffffu, here) && ok;
-        }
-    };
-    auto used = [&]() {
-        pending = max(0, pending - 1);
-        if (++take == RING) { take = 0; phase ^= 1; }
-    };
+    uint4 kr[4][2][KC], vr[KS][2];
+    auto load_k = [&](int id) {       // a block that is not there: block 0 is loaded and masked
+        const unsigned char* base = p.kcache + (size_t)max(id, 0) * (C8_BLOCK * D) + (g & 1) * D + 16 * t;
 #pragma unroll
-    for (int u = 0; u < RING; ++u) ask(u & 3);
-    if (!short_first) look_behind();
-
-    int count = 0;
-    A8Piece w;
-    while (a8_next(p, meta, cur, w)) {
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int c = 0; c < KC; ++c) kr[j][h][c] = a8_load(base + (4 * j + 2 * h) * D + 64 * c);
+    };
+    auto load_v = [&](int id) {       // id: of block t
+        const unsigned char* base = p.vcache + (size_t)max(id, 0) * (C8_BLOCK * D) + g * C8_BLOCK;
+#pragma unroll
+        for (int m = 0; m < KS; ++m)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) vr[m][h] = a8_load(base + (16 * m + 8 * h) * C8_BLOCK);
+    };
+    A8Cursor cur;
+    a8_begin(p, meta, cta_from + of_warps.from(warp), cta_from + of_warps.from(warp + 1), cur);
+    A8Piece w, following;
+    bool valid = a8_next(p, meta, cur, w);
+    int id = 0;
+    float ks = 0.0f, vs = 0.0f;
+    if (valid) {
+        id = lookup(w, w.tile);
+        load_k(id);
+        load_v(__shfl_sync(0xffffffffu, id, 8 * t));
+        ks = p.kscale[max(id, 0)]; vs = p.vscale[max(id, 0)];
+    }
+    while (valid) {
+        const bool have_next = a8_next(p, meta, cur, following);
         const int row = meta.row[w.seg];
         // queries of head g as the second operand, scaled by a power of two into [1, 2); lanes of heads that are not: zeros
         unsigned qb[KS][2];
@@ -414,42 +319,31 @@ __global__ void __launch_bounds__(A8_THREADS, 1) attn_decode_8bit_kernel(const A
         float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
 
 #pragma unroll 1
-        for (int tile = w.tile; tile < w.tile + w.ntiles; ++tile) {
+        for (int left = w.ntiles, tile = w.tile; left > 0; --left, ++tile) {
+            const bool more = left > 1 || have_next;
+            const int id_next = left > 1 ? lookup(w, tile + 1) : have_next ? lookup(following, following.tile) : -1;
+            float ks_next = 0.0f, vs_next = 0.0f;
             float s[4][4];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                arrived();
-                uint4 kr[2][2][KC];
-                const unsigned char* rows = sh.ring[warp] + take * UNIT + (g >> 1) * Shared::PITCH + (g & 1) * D + 16 * t;
+            for (int j = 0; j < 4; ++j) { s[j][0] = 0.0f; s[j][1] = 0.0f; s[j][2] = 0.0f; s[j][3] = 0.0f; }
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
+            for (int k = 0; k < KS; ++k) {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int c = 0; c < KC; ++c) kr[i][h][c] = *reinterpret_cast<const uint4*>(rows + (4 * i + 2 * h) * D + 64 * c);
-                used();
-                ask((u + RING) & 3);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) s[2 * u + i / 4][i % 4] = 0.0f;
-#pragma unroll
-                for (int k = 0; k < KS; ++k)                 // two sums in turn: a product waits for the one before in its sum
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        unsigned a0, a1, a2, a3;
-                        c8_decode4<E4M3>(a8_word(kr[i][0][k / 4], k % 4), a0, a2);
-                        c8_decode4<E4M3>(a8_word(kr[i][1][k / 4], k % 4), a1, a3);
-                        a8_mma(s[2 * u + i], a0, a1, a2, a3, qb[k][0], qb[k][1]);
-                    }
+                for (int j = 0; j < 4; ++j) {
+                    unsigned a0, a1, a2, a3;
+                    c8_decode4<E4M3>(a8_word(kr[j][0][k / 4], k % 4), a0, a2);
+                    c8_decode4<E4M3>(a8_word(kr[j][1][k / 4], k % 4), a1, a3);
+                    a8_mma(s[j], a0, a1, a2, a3, qb[k][0], qb[k][1]);
+                }
             }
-            const int at = count++ & (Shared::TILES - 1);
-            a8_wait_group<(RING + 1) / 4>();               // this tile's scales; those of the tiles asked for since may be under way
-            __syncwarp();
-            const int id = sh.id[warp][at][g >> 1];
-            const float ks = sh.ks[warp][at][g >> 1];
+            if (more) {
+                load_k(id_next);
+                ks_next = p.kscale[max(id_next, 0)]; vs_next = p.vscale[max(id_next, 0)];
+            }
             // ---- softmax: all rows of a lane lie in block g >> 1 -------------------------------------------------
             const int base = tile * A8_TILE;
             const bool full = base >= w.lo && base + A8_TILE - 1 <= w.pos && __all_sync(0xffffffffu, id >= 0);
-            const float vs = fmaxf(sh.vs[warp][at][g >> 1], 8.673617379884035e-19f);      // 2^-60: a scale of zero still counts in the sum
+            vs = fmaxf(vs, 8.673617379884035e-19f);      // 2^-60: a scale of zero still counts in the sum
             const float lv = log2f(vs), c0 = f0 * ks, c1 = f1 * ks;
             float x0 = -INFINITY, x1 = -INFINITY;
 #pragma unroll
@@ -494,47 +388,38 @@ __global__ void __launch_bounds__(A8_THREADS, 1) attn_decode_8bit_kernel(const A
                     pb[j][h] = a8_turn(*reinterpret_cast<const unsigned*>(&v));
                 }
             l0 = fmaf(t0, back, l0); l1 = fmaf(t1, back, l1);
-            unsigned mask[4];
             if (!full) {                   // whatever lies in the value bytes of hidden keys must not meet a weight of zero
                 const int begin = base + t * C8_BLOCK;
                 const bool there = __shfl_sync(0xffffffffu, id, 8 * t) >= 0;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    mask[j] = 0u;
+                    unsigned mask = 0u;
 #pragma unroll
                     for (int b = 0; b < 4; ++b) {
                         const int key = begin + 4 * j + b;
-                        mask[j] |= (there && key >= w.lo && key <= w.pos) ? 0xffu << (8 * b) : 0u;
+                        mask |= (there && key >= w.lo && key <= w.pos) ? 0xffu << (8 * b) : 0u;
                     }
+#pragma unroll
+                    for (int m = 0; m < KS; ++m)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            if (j == 0) vr[m][h].x &= mask; else if (j == 1) vr[m][h].y &= mask;
+                            else if (j == 2) vr[m][h].z &= mask; else vr[m][h].w &= mask;
+                        }
                 }
             }
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                arrived();
-                uint4 vr[KS / 2][2];
-                const unsigned char* lines = sh.ring[warp] + take * UNIT + t * Shared::PITCH + g * C8_BLOCK;
+            for (int j = 0; j < 4; ++j) {
 #pragma unroll
-                for (int x = 0; x < KS; ++x) vr[x / 2][x % 2] = *reinterpret_cast<const uint4*>(lines + (x * 8) * C8_BLOCK);
-                used();
-                ask((u + 2 + RING) & 3);
-                if (!full) {
-#pragma unroll
-                    for (int x = 0; x < KS; ++x) {
-                        vr[x / 2][x % 2].x &= mask[0]; vr[x / 2][x % 2].y &= mask[1];
-                        vr[x / 2][x % 2].z &= mask[2]; vr[x / 2][x % 2].w &= mask[3];
-                    }
-                }
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-#pragma unroll
-                    for (int m = 0; m < KS / 2; ++m) {
-                        unsigned a0, a1, a2, a3;
-                        c8_decode4<E4M3>(a8_word(vr[m][0], j), a0, a2);
-                        c8_decode4<E4M3>(a8_word(vr[m][1], j), a1, a3);
-                        a8_mma(o[u * (KS / 2) + m], a0, a1, a2, a3, pb[j][0], pb[j][1]);
-                    }
+                for (int m = 0; m < KS; ++m) {
+                    unsigned a0, a1, a2, a3;
+                    c8_decode4<E4M3>(a8_word(vr[m][0], j), a0, a2);
+                    c8_decode4<E4M3>(a8_word(vr[m][1], j), a1, a3);
+                    a8_mma(o[m], a0, a1, a2, a3, pb[j][0], pb[j][1]);
                 }
             }
+            if (more) load_v(__shfl_sync(0xffffffffu, id_next, 8 * t));
+            id = id_next; ks = ks_next; vs = vs_next;
         }
         // ---- the end of the piece -----------------------------------------------------------------------------------------
 #pragma unroll
@@ -575,13 +460,14 @@ __global__ void __launch_bounds__(A8_THREADS, 1) attn_decode_8bit_kernel(const A
             }
             float* p0 = sh.part(warp, w.begins, 2 * t);
             float* p1 = sh.part(warp, w.begins, 2 * t + 1);
-            __syncwarp();                                 // the queue is no longer read
 #pragma unroll
             for (int m = 0; m < KS; ++m) {
                 p0[16 * m + g] = o[m][0]; p1[16 * m + g] = o[m][1];
                 p0[16 * m + 8 + g] = o[m][2]; p1[16 * m + 8 + g] = o[m][3];
             }
         }
+        valid = have_next;
+        w = following;
     }
     // (The next kernel is not let in early: with a pdl_trigger() here the product behind this
     // kernel spreads unevenly over the SMs that end first, and a decode step of 36 layers goes from 3.9 to 6.3 ms.)
@@ -742,16 +628,4 @@ PI_EXPORT int pi_attention_decode_8bit(const A8Args* args, cudaStream_t stream) 
     if (units > 1000000000LL) return pi_refuse("pi_attention_decode_8bit: up to %lld tiles of keys are beyond the limit", units);
     if (head_dim == 128) return cache_dtype == PI_E4M3 ? a8_launch<128, true>(p, ws_ctas, stream) : a8_launch<128, false>(p, ws_ctas, stream);
     return cache_dtype == PI_E4M3 ? a8_launch<64, true>(p, ws_ctas, stream) : a8_launch<64, false>(p, ws_ctas, stream);
-}
-
-// 0 if every wait of the launches so far was met, else a code of the first that ran out (reading resets it)
-PI_EXPORT int pi_attention_8bit_status(unsigned* status) {
-    unsigned zero = 0;
-    cudaError_t err = cudaMemcpyFromSymbol(status, g_a8_status, sizeof(unsigned));
-    if (err == cudaSuccess) err = cudaMemcpyToSymbol(g_a8_status, &zero, sizeof(unsigned));
-    if (err != cudaSuccess) {
-        snprintf(g_pi_error, sizeof(g_pi_error), "pi_attention_8bit_status: %s", cudaGetErrorString(err));
-        return (int)err;
-    }
-    return 0;
 }

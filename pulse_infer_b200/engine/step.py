@@ -114,6 +114,3 @@ class ModelRunner:
             status = ops.attention_tcgen05_loaded_status()
             if status:
                 raise StepError(f"a wait inside the tcgen05 attention kernel ran out (status {status:#x})")
-            status = ops.attention_8bit_status()
-            if status:
-                raise StepError(f"a wait inside the decode attention over 8-bit pages ran out (status {status:#x})")

@@ -294,13 +294,3 @@ def attention_prompt_8bit(q: torch.Tensor, q_stride: int, kcache: torch.Tensor, 
     return attention_tcgen05(q, q_stride, keys, values, maps.table, maps.seg_off, maps.rows, seg_start, seg_len, num_tokens, R,
                              longest, nq, nkv, d, page_size, window, scale, out, splits=splits, part_acc=acc, part_ml=ml,
                              token_seg=maps.token_seg)
-
-
-def attention_8bit_status() -> int:
-    """0 if every bounded wait of the decode kernel's launches so far was met (synchronises the device); 0 if it is not loaded."""
-    lib = _k._LIBS.get(("attention_8bit", None))
-    if lib is None:
-        return 0
-    status = ctypes.c_uint(0)
-    _k._check(lib, lib.pi_attention_8bit_status(ctypes.byref(status)), "attention_8bit_status", launches=0)
-    return int(status.value)

@@ -518,50 +518,6 @@ def test_what_the_cache_kernels_refuse():
         _refused(lambda: ops.attention_prompt_8bit(**{**base, **kw}))
 
 
-def test_a_wait_that_runs_out_is_reported_and_the_next_launch_works(monkeypatch, model_folders):
-    """The give-up path of the decode kernel's bounded waits, in a test build (a small poll limit; the second tile of one
-    warp lacks one copy, so its unit never arrives): the launch returns, the status names the warp and the unit, the step
-    function's check raises, and the regular build is right afterwards.  Nothing traps or spins without a limit, and no
-    copy is in flight when the kernel ends (the missing one is never started, the others are waited for)."""
-    import ctypes
-    dev, ops = need_gpu(), _ops()
-    from pulse_infer_b200.csrc import build
-    from pulse_infer_b200.engine import StepError
-    from test_gpu_engine import _runner
-    ops.kernels._lib("attention_8bit")
-    monkeypatch.setenv("PULSE_NVCC_FLAGS", "-DA8_TEST_HOOKS -DA8_SPIN_LIMIT=65536")
-    test_lib = ctypes.CDLL(build.library_path("attention_8bit"))
-    monkeypatch.delenv("PULSE_NVCC_FLAGS")
-    test_lib.pi_last_error.restype = ctypes.c_char_p
-    runner = _runner(model_folders["E"], "bfloat16", cache_dtype="int8")
-    assert ops.attention_8bit_status() == 0
-    ws = ops.attention_decode_workspace(128, dev)
-    with monkeypatch.context() as m:
-        m.setitem(ops.kernels._LIBS, ("attention_8bit", None), test_lib)
-        _decode(ops, dev, torch.int8, [60], 4, 1, 128, 16, workspace=ws)            # one tile: the left-out copy is not reached
-        assert ops.attention_8bit_status() == 0
-        for _ in range(2):
-            seqs = Sequences([1600], 1, 128, 16, torch.int8)
-            meta = segments_to_device([(0, 1599, 1)], dev)
-            ops.attention_decode_8bit(torch.zeros(1, 512, dtype=torch.bfloat16, device=dev), 512, *seqs.pools.on(dev), seqs.table.to(dev),
-                                      meta["seg_off"], meta["seg_slot"], meta["seg_start"], meta["seg_len"], 1, 1, 4, 1, 128, None, 0.1,
-                                      workspace=ws, span_min=1000)
-            torch.cuda.synchronize()                                              # the kernel gave up and returned
-            # block 0, warp 1; its second tile's first unit of values is the seventh of its queue of five: place 1
-            assert ops.attention_8bit_status() == 0x8b000000 | (0 << 8) | (1 << 4) | 1
-            assert not ws.count.any()
-        ops.attention_decode_8bit(torch.zeros(1, 512, dtype=torch.bfloat16, device=dev), 512, *seqs.pools.on(dev), seqs.table.to(dev),
-                                  meta["seg_off"], meta["seg_slot"], meta["seg_start"], meta["seg_len"], 1, 1, 4, 1, 128, None, 0.1,
-                                  workspace=ws, span_min=1000)
-        torch.cuda.synchronize()
-        with pytest.raises(StepError, match="8-bit pages"):
-            runner.check_device_errors()
-        assert ops.attention_8bit_status() == 0
-    _decode(ops, dev, torch.int8, [1600], 4, 1, 128, 16, workspace=ws)
-    assert ops.attention_8bit_status() == 0
-    runner.check_device_errors()
-
-
 @pytest.mark.parametrize("requests", [257, 1024])
 def test_decode_a_great_many_short_requests(requests):
     """More requests than threads in a block, most of them a tile or two long, some of no length at all."""
