@@ -1441,32 +1441,45 @@ PI_EXPORT int pi_attention_tcgen05_supported(int page_size) {
     return page_size == 8 || page_size == 16 || page_size == 32 || page_size == 64 || page_size == 128;
 }
 
+// arguments as one record of 8-byte fields
+struct FaArgs {
+    const void* q; long long q_stride; const void* kcache; const void* vcache; long long num_pages;
+    const int* block_table; long long bt_stride; const int* seg_off; const int* seg_slot; const int* seg_start; const int* seg_len;
+    void* out; long long num_segments, max_seg_len, nq, nkv, page_size, window, splits;
+    float* part_acc; float* part_ml; const int* token_seg; long long num_tokens;
+    double scale;
+};
+
 // Prompt portions only: segments of one token are skipped (run the decode kernel for those).
-PI_EXPORT int pi_attention_tcgen05(const void* q, int q_stride, const void* kcache, const void* vcache, long long num_pages,
-                                   const int* block_table, int bt_stride, const int* seg_off, const int* seg_slot,
-                                   const int* seg_start, const int* seg_len, void* out, int num_segments, int max_seg_len,
-                                   int nq, int nkv, int page_size, int window, float scale, int splits, float* part_acc,
-                                   float* part_ml, const int* token_seg, int num_tokens, cudaStream_t stream) {
+PI_EXPORT int pi_attention_tcgen05(const FaArgs* args, cudaStream_t stream) {
+    const FaArgs& a = *args;
+    const int q_stride = (int)a.q_stride, bt_stride = (int)a.bt_stride, num_segments = (int)a.num_segments, max_seg_len = (int)a.max_seg_len;
+    const int nq = (int)a.nq, nkv = (int)a.nkv, page_size = (int)a.page_size, window = (int)a.window, splits = (int)a.splits;
+    const int num_tokens = (int)a.num_tokens;
+    const float scale = (float)a.scale;
+    const void *q = a.q, *kcache = a.kcache, *vcache = a.vcache;
+    void* out = a.out;
+    float *part_acc = a.part_acc, *part_ml = a.part_ml;
     if (num_segments <= 0 || max_seg_len <= 0) return 0;
     if (splits < 1 || splits > 64) return pi_refuse("pi_attention_tcgen05: splits=%d must be 1..64", splits);
-    if (splits > 1 && (part_acc == nullptr || part_ml == nullptr || token_seg == nullptr || num_tokens <= 0))
+    if (splits > 1 && (part_acc == nullptr || part_ml == nullptr || a.token_seg == nullptr || num_tokens <= 0))
         return pi_refuse("pi_attention_tcgen05: key splitting needs its scratch, the token-to-segment table and the token count");
-    if (splits > 1 && (((uintptr_t)part_acc & 15) || ((uintptr_t)part_ml & 7) || ((uintptr_t)out & 7)))
-        return pi_refuse("pi_attention_tcgen05: the scratch of key splitting must start on 16-byte boundaries, the output on 8-byte ones");
+    if (splits > 1 && (((uintptr_t)part_acc & 15) || ((uintptr_t)part_ml & 7)))
+        return pi_refuse("pi_attention_tcgen05: the scratch of key splitting must start on 16-byte boundaries");
     if (!(scale > 0.0f)) return pi_refuse("pi_attention_tcgen05: the score scale must be positive");
     if (nq <= 0 || nkv <= 0 || nq % nkv != 0) return pi_refuse("pi_attention_tcgen05: nq=%d must be a positive multiple of nkv=%d", nq, nkv);
     if (!pi_attention_tcgen05_supported(page_size)) return pi_refuse("pi_attention_tcgen05: page size %d is not one of 8, 16, 32, 64, 128", page_size);
-    if (q_stride % 8 != 0 || ((uintptr_t)q & 15) || ((uintptr_t)kcache & 127) || ((uintptr_t)vcache & 127))
-        return pi_refuse("pi_attention_tcgen05: q must be 16-byte aligned with a stride that is a multiple of 8, pages 128-byte aligned");
+    if (q_stride % 8 != 0 || ((uintptr_t)q & 15) || ((uintptr_t)out & 15) || ((uintptr_t)kcache & 127) || ((uintptr_t)vcache & 127))
+        return pi_refuse("pi_attention_tcgen05: q and the output must be 16-byte aligned, q with a stride that is a multiple of 8, pages 128-byte aligned");
     CUtensorMap mk, mv;
-    const long long rows = num_pages * nkv * page_size;
+    const long long rows = a.num_pages * nkv * page_size;
     int rc = fa_make_map(&mk, kcache, rows, page_size);
     if (rc) return rc;
     rc = fa_make_map(&mv, vcache, rows, page_size);
     if (rc) return rc;
     FaParams p;
-    p.q = (const bf16*)q; p.q_stride = q_stride; p.block_table = block_table; p.bt_stride = bt_stride;
-    p.seg_off = seg_off; p.seg_slot = seg_slot; p.seg_start = seg_start; p.seg_len = seg_len;
+    p.q = (const bf16*)q; p.q_stride = q_stride; p.block_table = a.block_table; p.bt_stride = bt_stride;
+    p.seg_off = a.seg_off; p.seg_slot = a.seg_slot; p.seg_start = a.seg_start; p.seg_len = a.seg_len;
     p.out = (bf16*)out; p.nq = nq; p.nkv = nkv; p.group = nq / nkv; p.page_size = page_size; p.window = window;
     p.scale_log2 = scale * 1.4426950408889634f;
     p.tiles_per_seg = (int)(((long long)max_seg_len * p.group + FA_ROWS - 1) / FA_ROWS);
@@ -1474,24 +1487,26 @@ PI_EXPORT int pi_attention_tcgen05(const void* q, int q_stride, const void* kcac
     p.splits = splits; p.part_acc = part_acc; p.part_ml = part_ml;
     const long long ctas = (long long)num_segments * p.tiles_per_seg * nkv;
     if (ctas > 2147483647LL) return pi_refuse("pi_attention_tcgen05: %lld tiles are beyond the grid limit", ctas);
-    static bool configured = false;
+    static bool configured[64] = {};                          // per device: the attribute belongs to a device's copy of the kernel
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return pi_refuse("pi_attention_tcgen05: no current device below 64");
     constexpr unsigned tile_bytes = (PI_HEAD_DIM / 64) * 128 * 128;
     const size_t smem = (size_t)(2 + FA_STAGES) * tile_bytes + (2 * FA_STAGES + 6) * 8 + 16 + 1024;
     auto kernel = attn_tcgen05_kernel<PI_HEAD_DIM>;
-    if (!configured) {
+    if (!configured[device]) {
         cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (err != cudaSuccess) {
             snprintf(g_pi_error, sizeof(g_pi_error), "pi_attention_tcgen05: cannot reserve %zu bytes of shared memory: %s", smem, cudaGetErrorString(err));
             return (int)err;
         }
-        configured = true;
+        configured[device] = true;
     }
     pi_launch(kernel, dim3((unsigned)ctas, (unsigned)splits), dim3(FA_THREADS), smem, stream, mk, mv, p);
     rc = pi_check_launch("pi_attention_tcgen05");
     if (rc || splits == 1) return rc;
     const long long merge_rows = (long long)num_tokens * nq;
     pi_launch(attn_prompt_merge_kernel<PI_HEAD_DIM>, dim3((unsigned)((merge_rows + FA_MERGE_WARPS - 1) / FA_MERGE_WARPS)), dim3(FA_MERGE_WARPS * 32), 0,
-              stream, (const float*)part_acc, (const float*)part_ml, splits, (bf16*)out, token_seg, seg_len, nq, merge_rows);
+              stream, (const float*)part_acc, (const float*)part_ml, splits, (bf16*)out, a.token_seg, a.seg_len, nq, merge_rows);
     return pi_check_launch("pi_attention_tcgen05 merge");
 }
 

@@ -16,8 +16,7 @@ from typing import NamedTuple
 import torch
 
 from . import kernels as _k
-from .kernels import (BF16, DecodeWorkspace, KernelError, _on_current_device, _Record, attention_tcgen05,
-                      choose_prompt_splits)
+from .kernels import BF16, DecodeWorkspace, KernelError, _on_current_device, _Record, choose_prompt_splits
 
 BLOCK_TOKENS = 16
 E4M3, INT8 = 2, 3
@@ -179,6 +178,11 @@ def qk_norm_rope_write_8bit(qkv: torch.Tensor, q_weight, k_weight, eps: float, c
     return q_out
 
 
+def _check_copy(name: str, t: torch.Tensor, N: int, nkv: int, page_size: int, d: int) -> None:
+    if t.dtype != torch.bfloat16 or t.dim() != 4 or t.shape[0] < N or tuple(t.shape[1:]) != (nkv, page_size, d) or not t.is_contiguous():
+        raise KernelError(f"{name} must be contiguous bfloat16 [at least {N}, {nkv}, {page_size}, {d}]")
+
+
 def pages_8bit_to_bf16(kcache: torch.Tensor, vcache: torch.Tensor, kscale: torch.Tensor, vscale: torch.Tensor,
                        page_list: torch.Tensor, page_tokens: torch.Tensor | None = None, keys: torch.Tensor | None = None,
                        values: torch.Tensor | None = None) -> tuple:
@@ -195,8 +199,8 @@ def pages_8bit_to_bf16(kcache: torch.Tensor, vcache: torch.Tensor, kscale: torch
     for name, t in (("keys", keys), ("values", values)):
         if t is None:
             t = torch.empty((N, nkv, page_size, d), dtype=torch.bfloat16, device=kcache.device)
-        elif t.dtype != torch.bfloat16 or t.dim() != 4 or t.shape[0] < N or tuple(t.shape[1:]) != (nkv, page_size, d) or not t.is_contiguous():
-            raise KernelError(f"{name} must be contiguous bfloat16 [at least {N}, {nkv}, {page_size}, {d}]")
+        else:
+            _check_copy(name, t, N, nkv, page_size, d)
         out.append(t)
     _READ(device, (kcache.data_ptr(), vcache.data_ptr(), kscale.data_ptr(), vscale.data_ptr(), code, pages, nkv, page_size, d,
                    page_list.data_ptr(), 0 if page_tokens is None else page_tokens.data_ptr(), N, out[0].data_ptr(),
@@ -269,28 +273,48 @@ def attention_prompt_8bit(q: torch.Tensor, q_stride: int, kcache: torch.Tensor, 
     runs on the copies.  ``portions``: (start, length) of the segments of more than one token, on the host.  ``keys`` /
     ``values``: bfloat16 [listed pages, kv heads, page size, d] for the copies, made here when missing; the layers of a step
     can share them.  Rows of single-token segments in ``out`` [num_tokens, nq d] are left as they are."""
-    _on_current_device((q, kcache, vcache, seg_start, seg_len, out, maps.table))
-    _, _, _, page_size, d = _check_pools(kcache, vcache, kscale, vscale, head_dim, nkv)
+    device = _on_current_device((q, kcache, vcache, kscale, vscale, seg_start, seg_len, out, keys, values, maps.page_list, maps.table))
+    code, pages, _, page_size, d = _check_pools(kcache, vcache, kscale, vscale, head_dim, nkv)
     if maps.table is None:
         raise KernelError("attention_prompt_8bit needs page maps with their table")
     out = _check_queries("attention_prompt_8bit", q, q_stride, num_tokens, nq, nkv, d, window, scale, out)
     R = maps.rows.numel()
     _vector("seg_start", seg_start, torch.int32, (R,))
     _vector("seg_len", seg_len, torch.int32, (R,))
-    longest = max((n for _, n in portions), default=0)
-    if longest < 2:
+    portions = [p for p in portions if p[1] > 1]
+    if not portions:
         return out
-    first = [max(0, a - window + 1) // page_size if window else 0 for a, _ in portions]
-    need = sum((a + n - 1) // page_size - f + 1 for (a, n), f in zip(portions, first) if n > 1)
+    longest = need = 0
+    for start, n in portions:
+        longest = max(longest, n)
+        first = max(0, start - window + 1) // page_size if window else 0
+        need += (start + n - 1) // page_size - first + 1
     if maps.page_list.numel() < need or maps.token_seg.numel() < num_tokens:
         raise KernelError(f"the page maps list {maps.page_list.numel()} pages and {maps.token_seg.numel()} tokens, the portions "
                           f"have {need} and {num_tokens}")
-    keys, values = pages_8bit_to_bf16(kcache, vcache, kscale, vscale, maps.page_list, maps.page_tokens, keys, values)
-    splits = choose_prompt_splits([p for p in portions if p[1] > 1], nq // nkv, nkv, window)
-    acc = ml = None
-    if splits > 1:
-        acc = torch.empty(num_tokens * nq * splits * d, dtype=torch.float32, device=q.device)
-        ml = torch.empty(num_tokens * nq * splits * 2, dtype=torch.float32, device=q.device)
-    return attention_tcgen05(q, q_stride, keys, values, maps.table, maps.seg_off, maps.rows, seg_start, seg_len, num_tokens, R,
-                             longest, nq, nkv, d, page_size, window, scale, out, splits=splits, part_acc=acc, part_ml=ml,
-                             token_seg=maps.token_seg)
+    N, W = maps.page_list.numel(), maps.table.shape[1]
+    _vector("page_list", maps.page_list, torch.int32, (N,))
+    _vector("page_tokens", maps.page_tokens, torch.int32, (N, 2))
+    _vector("table", maps.table, torch.int32, (R, W))
+    splits = choose_prompt_splits(portions, nq // nkv, nkv, window)
+    rows = num_tokens * nq * splits if splits > 1 else 0
+    # the copies and the shares' scratch in one allocation: pages are multiples of 2,048 bytes, a share's row of 256
+    pages_bytes = 2 * N * nkv * page_size * d
+    made = (keys is None) + (values is None)
+    scratch = torch.empty(made * pages_bytes + rows * (4 * d + 8), dtype=torch.uint8, device=q.device)
+    at = scratch.data_ptr()
+    where = []
+    for name, t in (("keys", keys), ("values", values)):
+        if t is None:
+            where.append(at)
+            at += pages_bytes
+        else:
+            _check_copy(name, t, N, nkv, page_size, d)
+            where.append(t.data_ptr())
+    _READ(device, (kcache.data_ptr(), vcache.data_ptr(), kscale.data_ptr(), vscale.data_ptr(), code, pages, nkv, page_size, d,
+                   maps.page_list.data_ptr(), maps.page_tokens.data_ptr(), N, where[0], where[1]), launches=1 if N else 0)
+    _k._PROMPT(device, (q.data_ptr(), q_stride, where[0], where[1], N, maps.table.data_ptr(), W, maps.seg_off.data_ptr(),
+                        maps.rows.data_ptr(), seg_start.data_ptr(), seg_len.data_ptr(), out.data_ptr(), R, longest, nq, nkv, page_size,
+                        window or 0, splits, at if rows else 0, at + rows * 4 * d if rows else 0, maps.token_seg.data_ptr(), num_tokens,
+                        scale), launches=2 if splits > 1 else 1, head_dim=d)
+    return out

@@ -105,13 +105,16 @@ class _Record:
         self.pack = struct.Struct(f"={fields}q{doubles}d").pack
         self.argtypes = (c_char_p,) + extra + (c_void_p,)
 
-    def __call__(self, device: int, args: tuple, extra: tuple = (), launches: int = 1) -> None:
-        lib = _LIBS.get((self.library, None)) or _lib(self.library)
+    def __call__(self, device: int, args: tuple, extra: tuple = (), launches: int = 1, head_dim: int | None = None) -> None:
+        lib = _LIBS.get((self.library, head_dim)) or _lib(self.library, head_dim)
         fn = getattr(lib, self.name)
         if fn.argtypes is None:
             fn.argtypes = self.argtypes
         stream = _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
         _check(lib, fn(self.pack(*args), *extra, stream), self.name, launches)
+
+
+_PROMPT = _Record("attention_tcgen05", "pi_attention_tcgen05", 23, 1)
 
 
 def _need_cuda(*tensors) -> None:
@@ -407,13 +410,12 @@ def attention_tcgen05(q: torch.Tensor, q_stride: int, kcache, vcache, block_tabl
         if (part_acc is None or part_ml is None or token_seg is None or part_acc.numel() < need * head_dim
                 or part_ml.numel() < need * 2 or part_acc.dtype != torch.float32 or part_ml.dtype != torch.float32):
             raise KernelError("scratch for the split prompt attention is missing or too small")
-    lib = _lib("attention_tcgen05", head_dim)
-    _check(lib, lib.pi_attention_tcgen05(
-        _p(q), c_int(q_stride), _p(kcache), _p(vcache), ctypes.c_longlong(kcache.shape[0]), _p(block_table),
-        c_int(block_table.shape[1]), _p(seg_off), _p(seg_slot), _p(seg_start), _p(seg_len), _p(out), c_int(num_segments),
-        c_int(max_seg_len), c_int(nq), c_int(nkv), c_int(page_size), c_int(window or 0), c_float(scale), c_int(splits),
-        _p(part_acc), _p(part_ml), _p(token_seg), c_int(num_tokens), _stream()),
-        "attention_tcgen05", launches=2 if splits > 1 else 1)
+    _PROMPT(_raw_device(), (q.data_ptr(), q_stride, kcache.data_ptr(), vcache.data_ptr(), kcache.shape[0], block_table.data_ptr(),
+                            block_table.shape[1], seg_off.data_ptr(), seg_slot.data_ptr(), seg_start.data_ptr(), seg_len.data_ptr(),
+                            out.data_ptr(), num_segments, max_seg_len, nq, nkv, page_size, window or 0, splits,
+                            part_acc.data_ptr() if splits > 1 else 0, part_ml.data_ptr() if splits > 1 else 0,
+                            token_seg.data_ptr() if splits > 1 else 0, num_tokens, scale),
+            launches=2 if splits > 1 else 1, head_dim=head_dim)
     return out
 
 
