@@ -61,7 +61,7 @@ struct FaParams {
     int nq, nkv, group;
     int page_size, window;
     float scale_log2;
-    int tiles_per_seg, num_segments;
+    int tiles_per_seg, num_segments, num_tokens;
     // key splitting for short portions behind long contexts: gridDim.y CTAs share the key tiles of a query block and
     // leave (reference point of the exponentials, sum, unnormalised output) per row for attn_prompt_merge_kernel
     int splits;
@@ -298,14 +298,15 @@ attn_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     const int rest = blockIdx.x / p.nkv;
     const int tile = p.tiles_per_seg - 1 - rest / p.num_segments;     // tiles with the most keys first
     const int seg = rest % p.num_segments;
-    const int len = p.seg_len[seg];
-    if (len == 1) return;                                 // single tokens go to the decode kernel
+    const int whole_len = p.seg_len[seg], tok_off = p.seg_off[seg];
+    if (whole_len == 1) return;                           // single tokens go to the decode kernel
+    const int len = min(whole_len, p.num_tokens - tok_off);          // tokens behind the last row of q and out are left out
     const int G = p.group;
     const int rows_total = len * G;
     const int row0 = tile * FA_ROWS;
     if (row0 >= rows_total) return;
     const bool two = row0 + FA_BM < rows_total;           // the second query tile has rows
-    const int start = p.seg_start[seg], tok_off = p.seg_off[seg];
+    const int start = p.seg_start[seg];
     const int* table = p.block_table + (size_t)p.seg_slot[seg] * p.bt_stride;
     const int row_last = min(row0 + FA_ROWS, rows_total) - 1;
     const int pos_first = start + row0 / G, pos_last = start + row_last / G;
@@ -402,7 +403,7 @@ attn_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         const unsigned page_bytes = (unsigned)ps * 128u;            // one (page, half) box
         auto lookup = [&](int j) -> int {
             const int key = kbegin + j * FA_BN + lane * ps;
-            return (j < num_tiles && lane < pages_per_tile && key < kend) ? table[key / ps] : -1;
+            return (j < num_tiles && lane < pages_per_tile && key < kend && key / ps < p.bt_stride) ? table[key / ps] : -1;
         };
         int page = lookup(0);
         for (int j = 0; j < num_tiles && !*failed; ++j) {
@@ -1483,7 +1484,7 @@ PI_EXPORT int pi_attention_tcgen05(const FaArgs* args, cudaStream_t stream) {
     p.out = (bf16*)out; p.nq = nq; p.nkv = nkv; p.group = nq / nkv; p.page_size = page_size; p.window = window;
     p.scale_log2 = scale * 1.4426950408889634f;
     p.tiles_per_seg = (int)(((long long)max_seg_len * p.group + FA_ROWS - 1) / FA_ROWS);
-    p.num_segments = num_segments;
+    p.num_segments = num_segments; p.num_tokens = num_tokens;
     p.splits = splits; p.part_acc = part_acc; p.part_ml = part_ml;
     const long long ctas = (long long)num_segments * p.tiles_per_seg * nkv;
     if (ctas > 2147483647LL) return pi_refuse("pi_attention_tcgen05: %lld tiles are beyond the grid limit", ctas);

@@ -272,7 +272,8 @@ def attention_prompt_8bit(q: torch.Tensor, q_stride: int, kcache: torch.Tensor, 
     (``page_maps(..., min_tokens=2)`` with the same window) are expanded to bfloat16, exactly, and the tcgen05 prompt kernel
     runs on the copies.  ``portions``: (start, length) of the segments of more than one token, on the host.  ``keys`` /
     ``values``: bfloat16 [listed pages, kv heads, page size, d] for the copies, made here when missing; the layers of a step
-    can share them.  Rows of single-token segments in ``out`` [num_tokens, nq d] are left as they are."""
+    can share them.  Rows of single-token segments in ``out`` [num_tokens, nq d] are left as they are, and segments' tokens
+    behind the first ``num_tokens`` are left out."""
     device = _on_current_device((q, kcache, vcache, kscale, vscale, seg_start, seg_len, out, keys, values, maps.page_list, maps.table))
     code, pages, _, page_size, d = _check_pools(kcache, vcache, kscale, vscale, head_dim, nkv)
     if maps.table is None:
@@ -288,7 +289,10 @@ def attention_prompt_8bit(q: torch.Tensor, q_stride: int, kcache: torch.Tensor, 
     for start, n in portions:
         longest = max(longest, n)
         first = max(0, start - window + 1) // page_size if window else 0
-        need += (start + n - 1) // page_size - first + 1
+        last = (start + n - 1) // page_size
+        need += last - first + 1
+        if start < 0 or last >= maps.table.shape[1]:
+            raise KernelError(f"a portion from {start} to {start + n - 1} is beyond a block table of {maps.table.shape[1]} pages of {page_size}")
     if maps.page_list.numel() < need or maps.token_seg.numel() < num_tokens:
         raise KernelError(f"the page maps list {maps.page_list.numel()} pages and {maps.token_seg.numel()} tokens, the portions "
                           f"have {need} and {num_tokens}")

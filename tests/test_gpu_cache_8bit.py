@@ -458,6 +458,40 @@ def test_a_step_of_portions_and_single_tokens(dtype, nq, nkv, d, page, window):
         t += n
 
 
+@pytest.mark.parametrize("fit", [1, 90, 200, 333])
+@pytest.mark.parametrize("start", [0, 5000])
+def test_portions_with_more_tokens_than_rows(fit, start):
+    # the maps, the queries and the output hold the first `fit` of 200 + 150 tokens: the others are left out, and nothing is
+    # written behind the last row (start 5000: with shares of the keys)
+    dev, ops = need_gpu(), _ops()
+    nq, nkv, d, page = 8, 2, 64, 16
+    portions = [(start, 200), (0, 150)]
+    g = torch.Generator().manual_seed(fit)
+    per = [(a + n + page - 1) // page for a, n in portions]
+    table = torch.full((2, max(per)), -1, dtype=torch.int32)
+    perm = torch.randperm(sum(per), generator=g).int()
+    table[0, :per[0]], table[1, :per[1]] = perm[:per[0]], perm[per[0]:]
+    pools = tuple(x.to(dev) for x in ops.cache_8bit_pools(sum(per), nkv, page, d, torch.int8, "cpu"))
+    pools[0].view(torch.uint8).random_(0, 256)
+    pools[1].view(torch.uint8).random_(0, 256)
+    for x in pools[2:]:
+        x.fill_(2.0 ** -6)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    s_, l_ = i32([a for a, _ in portions]), i32([n for _, n in portions])
+    q = torch.randn(350, nq * d, device=dev).to(torch.bfloat16)
+    results = []
+    for tokens in (350, fit):
+        maps = ops.page_maps(table.to(dev), i32([0, 1]), s_, l_, page, tokens, num_listed_pages=sum(per), min_tokens=2)
+        buffer = torch.full((352, nq * d), 7.0, dtype=torch.bfloat16, device=dev)
+        ops.attention_prompt_8bit(q[:tokens], nq * d, *pools, maps, s_, l_, portions, tokens, nq, nkv, d, None, d ** -0.5, out=buffer[:tokens])
+        assert ops.attention_tcgen05_loaded_status() == 0 and (buffer[tokens:] == 7).all()
+        results.append(buffer[:fit].double())
+    assert not (results[1] == 7).all(1).any()
+    # the shares of the keys may be cut elsewhere: weights and output round to bfloat16, twice each
+    bound = 4 * 2.0 ** -8 * pools[1].view(torch.int8).abs().max().item() * 2.0 ** -6
+    assert (results[0] - results[1]).abs().max().item() <= bound
+
+
 # ---- refusals ---------------------------------------------------------------------------------------------------------
 def _refused(call, *words):
     from pulse_infer_b200.ops import KernelError
