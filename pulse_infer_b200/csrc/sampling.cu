@@ -347,7 +347,7 @@ PI_EXPORT int pi_logit_edit(float* logits, int ld, int vocab, const int* rows, c
 // seen = v occurs in h, count = occurrences behind the prompt, for every token id v
 //   x = seen ? (x > 0 ? x / repetition : x * repetition) : x
 //   x = x - frequency * count - (seen ? presence : 0) + bias[v],   x = -inf where the row's mask has a zero bit
-// Of several biases of a row for one id the last counts; ids outside the vocabulary are passed over.
+// A bias of -inf forbids the id, whatever its logit is.  Of several biases of a row for one id the last counts; ids outside the vocabulary are passed over.
 //
 // The logits are read and written once (4 + 4 bytes each: what bounds a large step); a step of one row is bound by latency.
 // A block owns RULE_SLICE ids of a row.  It asks for their logits; while they come it counts the history's ids of its slice in
@@ -446,7 +446,10 @@ __global__ void __launch_bounds__(RULE_THREADS, 6) logit_rules_kernel(const Rule
             for (int c = 0; c < 4; ++c) {
                 const float changed = e[c] * (e[c] > 0.0f ? inv_rep : rep) - freq * (float)(mk[c] & 0x3fffffffu) - pres;
                 e[c] = (mk[c] & 0xbfffffffu) != 0u ? changed : e[c];
-                if (BIAS && (mk[c] & 0x40000000u)) e[c] += p.bias_values[bias_at[i + c] - 1];
+                if (BIAS && (mk[c] & 0x40000000u)) {
+                    const float bias = p.bias_values[bias_at[i + c] - 1];
+                    e[c] = bias == -INFINITY ? bias : e[c] + bias;          // forbidden, whatever the logit is
+                }
             }
         }
         const float4 o = make_float4(bits & 1u ? e[0] : -INFINITY, bits & 2u ? e[1] : -INFINITY, bits & 4u ? e[2] : -INFINITY,

@@ -854,7 +854,7 @@ def logit_rules(logits: torch.Tensor, history: torch.Tensor, history_off: torch.
     ``history[history_off[r]:history_off[r + 1]]`` (int32), its first ``prompt_len[r]`` entries the prompt.  In this order:
     a token of the history has its logit divided (if positive, else multiplied) by ``repetition[r]``; ``frequency[r]`` is
     subtracted for each occurrence behind the prompt, ``presence[r]`` once if it occurs at all; ``bias_values`` of
-    ``bias_tokens[bias_off[r]:bias_off[r + 1]]`` are added (the last of several for one token counts); tokens whose bit is
+    ``bias_tokens[bias_off[r]:bias_off[r + 1]]`` are added (the last of several for one token counts; -inf forbids it); tokens whose bit is
     zero in row ``mask_row[r]`` of ``mask`` (int32 [m, ceil(V / 32)], bit v % 32 of word v / 32; row -1, or one that is not
     there: all allowed) become -inf.  ids outside the vocabulary are passed over.  ``out`` may be ``logits`` itself."""
     device = _on_current_device((logits, history, history_off, prompt_len, repetition, frequency, presence, bias_off, bias_tokens,
@@ -884,6 +884,10 @@ def logit_rules(logits: torch.Tensor, history: torch.Tensor, history_off: torch.
         raise KernelError(f"logit_rules: out must be float32 [{n}, {V}] with unit stride and rows apart")
     ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
     ld, out_ld = (logits.stride(0), out.stride(0)) if n > 1 else (V, V)
+    apart = (out.data_ptr() - logits.data_ptr()) // 4
+    if not (apart == 0 and ld == out_ld) and -((n - 1) * out_ld + V) < apart < (n - 1) * ld + V \
+            and not (ld == out_ld and V <= apart % ld <= ld - V):
+        raise KernelError("logit_rules: out overlaps the logits without being the same")
     _LOGIT_RULES(device, (logits.data_ptr(), ld, out.data_ptr(), out_ld, n, V, history.data_ptr(),
                           history_off.data_ptr(), history.numel(), prompt_len.data_ptr(), repetition.data_ptr(), frequency.data_ptr(),
                           presence.data_ptr(), ptr(bias_off), ptr(bias_tokens), ptr(bias_values),

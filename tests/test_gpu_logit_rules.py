@@ -236,3 +236,29 @@ def test_logit_rules_rows_that_overlap_are_refused_and_one_row_may_have_any_stri
     odd = torch.empty_strided((1, V), (3, 1), device=dev)
     odd.copy_(src)
     assert torch.equal(ops.logit_rules(odd, *args), ops.logit_rules(src, *args))
+
+
+def test_a_bias_of_minus_infinity_forbids_whatever_the_logit_is():
+    dev, ops = need_gpu(), _ops()
+    x = torch.zeros(2, 40, device=dev)
+    x[0, 5], x[0, 6], x[0, 7], x[1, 5] = float("inf"), float("nan"), 2.0, float("inf")
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+    one, none = torch.ones(2, device=dev), torch.zeros(2, device=dev)
+    out = ops.logit_rules(x, i32([]), i32([0, 0, 0]), i32([0, 0]), one, none, none, bias_off=i32([0, 3, 3]), bias_tokens=i32([5, 6, 7]),
+                          bias_values=torch.full((3,), -float("inf"), device=dev))
+    assert (out[0, 5:8] == -float("inf")).all() and (out[0, :5] == 0).all() and (out[0, 8:] == 0).all() and out[1, 5] == float("inf")
+
+
+def test_logit_rules_output_that_overlaps_the_logits():
+    from pulse_infer_b200.ops import KernelError
+    dev, ops = need_gpu(), _ops()
+    i32 = lambda n: torch.zeros(n, dtype=torch.int32, device=dev)  # noqa: E731
+    rules = (i32(0), i32(4), i32(3), torch.ones(3, device=dev), torch.zeros(3, device=dev), torch.zeros(3, device=dev))
+    flat = torch.randn(1000, device=dev)
+    view = lambda at, ld: flat.as_strided((3, 70), (ld, 1), at)  # noqa: E731
+    for a, b in (((0, 80), (1, 80)), ((4, 80), (0, 80)), ((0, 80), (0, 90)), ((0, 80), (200, 80)), ((100, 200), (31, 200)), ((0, 70), (139, 70))):
+        with pytest.raises(KernelError):
+            ops.logit_rules(view(*a), *rules, out=view(*b))
+    for a, b in (((0, 80), (0, 80)), ((0, 200), (70, 200)), ((100, 200), (30, 200)), ((0, 70), (210, 70)), ((300, 80), (60, 80))):
+        want = view(*a).clone()
+        assert torch.equal(ops.logit_rules(view(*a), *rules, out=view(*b)), want)
