@@ -552,6 +552,29 @@ def test_what_the_cache_kernels_refuse():
         _refused(lambda: ops.attention_prompt_8bit(**{**base, **kw}))
 
 
+def test_outputs_off_their_boundaries_are_refused():
+    dev, ops = need_gpu(), _ops()
+    nq, nkv, d, page = 2, 1, 64, 16
+    pools = ops.cache_8bit_pools(4, nkv, page, d, torch.int8, dev)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    table, start, length = i32(0, 1).view(1, 2), i32(0), i32(3)
+    maps = ops.page_maps(table, i32(0), start, length, page, 3, num_listed_pages=1, min_tokens=2)
+    buffer = torch.zeros(4 * nq * d, dtype=torch.bfloat16, device=dev)
+    q = torch.randn(3, nq * d, device=dev).to(torch.bfloat16)
+    for off, prompt, decode in ((0, True, True), (8, True, True), (4, False, True), (1, False, False), (2, False, False)):
+        out = buffer[off:off + 3 * nq * d].view(3, nq * d)
+        call = lambda: ops.attention_prompt_8bit(q, nq * d, *pools, maps, start, length, [(0, 3)], 3, nq, nkv, d, None, 0.1, out=out)  # noqa: E731
+        call() if prompt else _refused(call, "16-byte")
+        one = buffer[off:off + nq * d].view(1, nq * d)
+        call = lambda: ops.attention_decode_8bit(q[:1], nq * d, *pools, table, maps.seg_off, i32(0), start, i32(1), 1, 1, nq, nkv, d, None,  # noqa: E731
+                                                 0.1, out=one)
+        call() if decode else _refused(call, "8-byte")
+    torch.cuda.synchronize()
+    keys = torch.zeros(8 + nkv * page * d, dtype=torch.bfloat16, device=dev)
+    _refused(lambda: ops.pages_8bit_to_bf16(*pools, i32(0), keys=keys[1:1 + nkv * page * d].view(1, nkv, page, d)), "16-byte")
+    _refused(lambda: ops.attention_prompt_8bit(q, nq * d, *pools, maps, start, length, [(30, 3)], 3, nq, nkv, d, None, 0.1), "beyond a block table")
+
+
 @pytest.mark.parametrize("requests", [257, 1024])
 def test_decode_a_great_many_short_requests(requests):
     """More requests than threads in a block, most of them a tile or two long, some of no length at all."""
