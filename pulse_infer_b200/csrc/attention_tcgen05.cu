@@ -20,7 +20,7 @@
 // keeps them in turns; with a thread for each they fell into step, both in the softmax and then both at the tensor
 // pipe (2,039 tokens: 65.6 us against 57.7 at that stage).
 //
-// Measured (32 query / 8 kv heads of 128, pages of 16): 2,039 tokens 44.7 us; 8,192 tokens 470 to 520 us (1.05 to
+// Measured (32 query / 8 kv heads of 128, pages of 16): 2,039 tokens 44.7 us; 8,192 tokens 470 to 520 us (1.06 to
 // 1.17 PFLOP/s over the causal half, by the clock); 8 portions of 1,024 tokens 127 us; 128 tokens behind 16,384 in
 // nine shares 44.7 us with the merge.  A tile of 128 keys for both query tiles takes 1.9 to 2.1 us, of which the
 // tensor pipe needs 1.2; each CTA has 4 us before its first scores and 2.7 us behind its last ones.

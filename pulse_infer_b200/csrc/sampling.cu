@@ -353,14 +353,16 @@ PI_EXPORT int pi_logit_edit(float* logits, int ld, int vocab, const int* rows, c
 // A block owns RULE_SLICE ids of a row.  It asks for their logits; while they come it counts the history's ids of its slice in
 // shared memory (every block of the row walks the whole history out of L2; integer atomics, so the order does not matter), and
 // applies the rules as it stores.  No workspace, no second launch.
-// Measured (B200, 152k logits): 3.4 us for a row with a history of 4,000; 24 us for 64 rows with histories to 8,000, 300 biases
-// and masks (12.2 us of traffic; 11.3 us without any rule, so the walks and marks are the rest).  Tried and slower there: the
+// Measured (B200, 152k logits): 3.3 us for a row with a history of 4,000; 23 us for 64 rows with histories to 8,000, 300 biases
+// and masks (12.2 us of traffic; 11.5 us without any rule, so the walks and marks are the rest).  Slices of 4,096 ids for 256
+// threads: 3.5 and 24.4 us (more walks); 8,192 for 512, with 64 KB of shared memory: 3.5 and 22.3 us; 12,288 for 768: 4.1 and
+// 23.9; the first history entries asked for before the logits: 23.9.  Tried and slower: the
 // history walked once by a cluster of eight blocks that mark through distributed shared memory (32 us); a copy kernel and a
 // second one with a block per 49,152 ids that changes only the marked ids (28 us); several slices one after the other in a
 // block (48 us); divisions by the penalty instead of products with its reciprocal (29 us: nearly every warp has a marked id).
 // ---------------------------------------------------------------------------------------------------
-#define RULE_THREADS 256
-#define RULE_SLICE 4096
+#define RULE_THREADS 384
+#define RULE_SLICE 6144
 #define RULE_VECS (RULE_SLICE / 4 / RULE_THREADS)
 #define RULE_BATCH 8            // history entries a thread has in flight
 
@@ -388,7 +390,7 @@ __device__ __forceinline__ void rule_walk(const int* history, int from, int to, 
 }
 
 template <bool BIAS>
-__global__ void __launch_bounds__(RULE_THREADS, 6) logit_rules_kernel(const RuleParams p) {
+__global__ void __launch_bounds__(RULE_THREADS, 4) logit_rules_kernel(const RuleParams p) {
     __shared__ __align__(16) unsigned mark[RULE_SLICE];        // bit 31: in the prompt, bit 30: has a bias; below: count behind it
     __shared__ __align__(16) int bias_at[BIAS ? RULE_SLICE : 4];   // index + 1 of the last bias for the id
     pdl_wait();

@@ -80,7 +80,7 @@ def _tensors(dev, V, histories, prompts, rep, freq, pres, biases, masks):
     return args, kw
 
 
-@pytest.mark.parametrize("rows,V", [(1, 151936), (5, 4096), (7, 4097), (3, 1), (6, 31), (9, 515), (5, 12291), (130, 2077)])
+@pytest.mark.parametrize("rows,V", [(1, 151936), (5, 4096), (7, 4097), (3, 1), (6, 31), (9, 515), (5, 12291), (130, 2077), (4, 6144), (4, 6145)])
 @pytest.mark.parametrize("with_bias,with_mask", [(True, True), (False, False), (True, False), (False, True)])
 def test_logit_rules(rows, V, with_bias, with_mask):
     dev, ops = need_gpu(), _ops()
