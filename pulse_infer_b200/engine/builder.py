@@ -63,6 +63,8 @@ def build_runner(model_dir: str | None = None, *, config=None, seed: int | None 
     model = build_model(config, runtime, **spec_options)
     if runtime.cache_dtype is not None:
         model.check_8bit_cache(page_size)
+        if max_requests > ops.PAGE_MAPS_MAX_SEGMENTS:
+            raise ValueError(f"an 8-bit cache takes at most {ops.PAGE_MAPS_MAX_SEGMENTS} requests, not {max_requests}")
     fast = runtime.mode == "bfloat16" and attention_impl != "simple"
     dims = head_dims_of(model)
     specs = [cs for cs in model.cache_specs() if cs is not None]

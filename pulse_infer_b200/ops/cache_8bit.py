@@ -210,6 +210,7 @@ def pages_8bit_to_bf16(kcache: torch.Tensor, vcache: torch.Tensor, kscale: torch
 
 # ---- attention ----------------------------------------------------------------------------------------------------------
 DECODE_8BIT_SPAN_MIN = 2      # shortest share of a CTA, in 64-key tiles and cost units
+DECODE_8BIT_MAX_SEGMENTS = 1024      # of a launch (A8_MAX_SEGS in csrc/attention_8bit.cu)
 DECODE_8BIT_PAIR_COST = 2     # units that a (request, kv head, eight query heads) triple counts for beside its tiles
 
 
@@ -242,6 +243,7 @@ def attention_decode_8bit(q: torch.Tensor, q_stride: int, kcache: torch.Tensor, 
     """Single tokens over 8-bit pages (csrc/attention_8bit.cu): segments of one token, whose keys and values - the newest
     included - are in the pages.  ``q`` holds the normalised, rotated query heads of token t at element offset t * q_stride.
     Rows of segments of several tokens in ``out`` [num_tokens, nq d] are left as they are (``attention_prompt_8bit``).
+    At most DECODE_8BIT_MAX_SEGMENTS segments; slices of the four seg_* tensors do for more.
     ``workspace`` (made here when missing): what CTAs leave for one another; launches that share one must not overlap."""
     device = _on_current_device((q, kcache, vcache, kscale, vscale, block_table, seg_off, seg_slot, seg_start, seg_len, out))
     code, pages, _, page_size, d = _check_pools(kcache, vcache, kscale, vscale, head_dim, nkv)

@@ -166,7 +166,10 @@ class Attention(Mixer):
                                       [(s.start, len(s.tokens)) for s in ctx.segments if len(s.tokens) > 1], ctx.num_tokens, nq, nkv,
                                       d, self.window, self.scale, out=out, keys=keys, values=values)
         if ctx.has_decode:
-            ops.attention_decode_8bit(q, nq * d, *pools, cache.block_table, ctx.seg_off, ctx.seg_slot, ctx.seg_start, ctx.seg_len,
-                                      ctx.num_tokens, ctx.num_segments, nq, nkv, d, self.window, self.scale,
-                                      workspace=ctx.decode_workspace(d), out=out)
+            most = ops.DECODE_8BIT_MAX_SEGMENTS
+            for at in range(0, ctx.num_segments, most):
+                segs = (ctx.seg_off, ctx.seg_slot, ctx.seg_start, ctx.seg_len) if ctx.num_segments <= most else \
+                    tuple(t[at:at + most] for t in (ctx.seg_off, ctx.seg_slot, ctx.seg_start, ctx.seg_len))
+                ops.attention_decode_8bit(q, nq * d, *pools, cache.block_table, *segs, ctx.num_tokens, min(most, ctx.num_segments - at),
+                                          nq, nkv, d, self.window, self.scale, workspace=ctx.decode_workspace(d), out=out)
         return out

@@ -172,6 +172,34 @@ def test_what_an_8bit_cache_refuses(model_folders):
         Engine(model_folders["C"], num_pages=8, cache_dtype="int8")
 
 
+def test_more_requests_than_a_decode_launch_takes(model_folders):
+    """1,030 requests decoding in one step, against the same in two steps of 515 (of which each is one launch a layer)."""
+    from pulse_infer_b200.engine import Segment
+    need_gpu()
+    vocab, R, logits = CONFIGS["D"].vocab_size, 1030, []
+    for cuts in ([R], [R // 2, R]):
+        runner = _runner(model_folders["D"], "int8", num_pages=R, max_requests=R, max_tokens_per_request=16)
+        for r in range(R):
+            runner.open(r)
+        for lo in range(0, R, 206):
+            runner.step([Segment(r, [(7 * r) % vocab, (11 * r + 3) % vocab, r % 5], []) for r in range(lo, lo + 206)])
+        rows, lo = [], 0
+        for hi in cuts:
+            rows.append(runner.step([Segment(r, [(13 * r) % vocab], [0]) for r in range(lo, hi)]).double().cpu())
+            lo = hi
+        runner.check_device_errors()
+        logits.append(torch.cat(rows))
+    _check(logits[0], logits[1].numpy(), logits[1].abs().max().item(), "int8", "one step against two")
+    assert (logits[1][:515] - logits[1][515:]).abs().max() > 0.5 * logits[1].abs().max()       # requests do differ
+
+
+def test_an_8bit_cache_for_more_requests_than_page_maps_take(model_folders):
+    need_gpu()
+    from pulse_infer_b200 import Engine
+    with pytest.raises(ValueError, match="at most 4096 requests"):
+        Engine(model_folders["E"], num_pages=8, cache_dtype="int8", max_batch_size=4097)
+
+
 def test_command_line_with_an_8bit_cache(model_folders):
     need_gpu()
     out = subprocess.run([sys.executable, os.path.join(ROOT, "bin", "qwen3_continuous_batch_demo"), model_folders["E"], "--prompt-len", "40",
