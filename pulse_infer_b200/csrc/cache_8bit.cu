@@ -21,8 +21,8 @@
 // rows went through the rotation tables of eight rows one after the other: 25 us instead of 12.)  A block looks for the
 // runs that begin among `window` tokens: 16 in a step of many tokens - one run, as a rule - and 1 in a decode step.  Query heads
 // are plain streaming work; in a step of many tokens they are a kernel of their own, in a small one part of the same launch.
-// Measured (B200, 32 + 8 + 8 heads of 128): 18 us for 2,045 tokens, both kernels, 46 MB (2.6 TB/s: too few loads in flight per
-// warp, as in the bf16 kernel); 2.9 us for 8 decoding requests.
+// Measured (B200, 32 + 8 + 8 heads of 128): 20.6 us for 2,045 tokens, both kernels, 46 MB (2.2 TB/s: too few loads in flight per
+// warp, as in the bf16 kernel, and the arithmetic of the keys); 3.1 us for 8 decoding requests.
 // ---------------------------------------------------------------------------------------------------
 #define CW_WARPS 4
 #define CW_Q_ROWS 4          // query rows in flight per lane group
@@ -127,6 +127,92 @@ __device__ __forceinline__ void cw_norm_rope(const CwParams& p, int sub, const f
     }
 }
 
+// a c + b s of numbers that are sums a + al and b + bl, as such a sum: rounding errors of products and sum are kept
+__device__ __forceinline__ float2 cw_dot2(float2 a, float c, float2 b, float s) {
+    // (intrinsics: nothing is to be drawn together here)
+    const float m = __fmul_rn(a.x, c), n = __fmul_rn(b.x, s), h = __fadd_rn(m, n), t = __fsub_rn(h, m);
+    const float sum_err = __fadd_rn(__fsub_rn(m, __fsub_rn(h, t)), __fsub_rn(n, t));
+    return make_float2(h, sum_err + (fmaf(a.x, c, -m) + fmaf(b.x, s, -n)) + fmaf(a.y, c, b.y * s));
+}
+
+// cw_norm_rope for a key row, to bf16.  A key is rounded to bf16 and then to its code, and one that lies close to the middle
+// between two codes falls to the other one if the errors before reach across it.  So the roundings of the norm and the rotation
+// are kept beside the value until its end: of 34 million keys none has another code than by the formula in 64 bits; with one
+// rounding after the other 21 had (19 with 32-bit arithmetic in torch).  It costs 2.6 us of 20.6 for 2,045 tokens.
+template <int D, bool ADJ>
+__device__ __forceinline__ uint4 cw_key_row(const CwParams& p, int sub, const float (&w)[8], const CwTurn<ADJ>& r, const uint4& raw) {
+    constexpr int LANES = D / 8;
+    float x[8];
+    cw_unpack(raw, x);
+    float2 v[8];
+    float inv = 1.0f, inv_err = 0.0f;
+    if (p.has_norm) {
+        float ss = 0.0f, ss_err = 0.0f;                      // the sum of squares and what its roundings left out
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float n = fmaf(x[k], x[k], ss);
+            ss_err += fmaf(x[k], x[k], __fsub_rn(ss, n));
+            ss = n;
+        }
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) {
+            const float other = __shfl_xor_sync(0xffffffffu, ss, o), n = __fadd_rn(ss, other), t = __fsub_rn(n, ss);
+            ss_err += __shfl_xor_sync(0xffffffffu, ss_err, o);
+            ss_err += __fadd_rn(__fsub_rn(ss, __fsub_rn(n, t)), __fsub_rn(other, t));
+            ss = n;
+        }
+        const float mean = ss * (1.0f / D), a = __fadd_rn(mean, p.eps), d = __fsub_rn(a, mean);
+        const float a_err = __fadd_rn(__fsub_rn(mean, __fsub_rn(a, d)), __fsub_rn(p.eps, d)) + ss_err * (1.0f / D);
+        inv = rsqrtf(a);
+        const float t = __fmul_rn(a, inv);                   // a step of Newton's: inv (1 + (1 - (a + a_err) inv^2) / 2)
+        inv_err = 0.5f * inv * (fmaf(-t, inv, 1.0f) - (fmaf(a, inv, -t) + a_err * inv) * inv);
+        if (!(fabsf(inv_err) <= inv)) inv_err = 0.0f;        // a is infinite, zero or no number
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { v[i].x = __fmul_rn(x[i], w[i]); v[i].y = fmaf(x[i], w[i], -v[i].x); }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = make_float2(x[i], 0.0f);
+    }
+    if (p.rot_pairs > 0) {
+        if constexpr (ADJ) {
+            if (4 * sub < p.rot_pairs) {
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    const float2 u = cw_dot2(v[2 * h], r.c[h], v[2 * h + 1], -r.s[h]);
+                    v[2 * h + 1] = cw_dot2(v[2 * h], r.s[h], v[2 * h + 1], r.c[h]);
+                    v[2 * h] = u;
+                }
+            }
+        } else {
+            const int shift = p.rot_pairs / 8;
+            const bool first = sub < shift, second = !first && sub < 2 * shift;
+            const int partner = first ? sub + shift : second ? sub - shift : sub;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float2 other = make_float2(__shfl_sync(0xffffffffu, v[i].x, partner, LANES), __shfl_sync(0xffffffffu, v[i].y, partner, LANES));
+                if (first || second) v[i] = cw_dot2(v[i], r.c[i], other, first ? -r.s[i] : r.s[i]);
+            }
+        }
+    }
+    uint4 out;
+    unsigned* half = reinterpret_cast<unsigned*>(&out);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float e[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const float2 u = v[2 * i + k];
+            const float m = __fmul_rn(u.x, inv);
+            float err = fmaf(u.x, inv, -m) + fmaf(u.x, inv_err, u.y * inv);
+            if (!(fabsf(err) <= fabsf(m))) err = 0.0f;       // of infinities
+            e[k] = m + err;
+        }
+        const __nv_bfloat162 pair = __floats2bfloat162_rn(e[0], e[1]);
+        half[i] = *reinterpret_cast<const unsigned*>(&pair);
+    }
+    return out;
+}
+
 // element i (0..7) of four registers of bf16 pairs
 __device__ __forceinline__ float cw_element(const uint4& raw, int i) {
     const unsigned w = i < 2 ? raw.x : i < 4 ? raw.y : i < 6 ? raw.z : raw.w;
@@ -207,10 +293,8 @@ __device__ __forceinline__ void cw_run(const CwParams& p, CwShared<D>& sh, int t
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
             const int i = row0 + r - off;
-            float x[8];
-            cw_unpack(row[r], x);
-            cw_norm_rope<D, ADJ>(p, sub, w, turn[r], x);
-            if (i >= 0 && i < count) row[r] = cw_pack(x);
+            const uint4 key = cw_key_row<D, ADJ>(p, sub, w, turn[r], row[r]);
+            if (i >= 0 && i < count) row[r] = key;
         }
     }
     float amax = 0.0f;

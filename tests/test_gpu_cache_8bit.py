@@ -232,6 +232,62 @@ def test_write_tokens_one_by_one_keep_the_formats_range(dtype):
                 assert ((got[t] * 2.0 ** e[-1] - true[t]).abs() <= room).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d,adjacent,weight_dtype", [(128, True, torch.bfloat16), (128, False, torch.float32), (64, False, torch.bfloat16)])
+def test_write_keys_have_the_codes_of_the_formula_in_64_bits(dtype, d, adjacent, weight_dtype):
+    """160 x 4 keys of d elements, rounded to 32 bits, to bfloat16 and to their codes: none may differ.  (What the kernel drops
+    before the first of these roundings is below 2^-40 of a value, so the chance that one differs is below 1e-6.)"""
+    dev, ops = need_gpu(), _ops()
+    T, nkv, page = 160, 4, 32
+    g = torch.Generator().manual_seed(d + adjacent)
+    qkv = torch.randn(T, 2 * nkv, d, generator=g).to(torch.bfloat16)
+    kw = (1 + 0.3 * torch.randn(d, generator=g)).to(weight_dtype)
+    angle = 100 * torch.rand(T, d // 2, generator=g).double()
+    cos, sin = angle.cos().float(), angle.sin().float()
+    k, v, ks, vs = ops.cache_8bit_pools(T // page, nkv, page, d, dtype, dev)
+    ops.qk_norm_rope_write_8bit(qkv.view(T, -1).to(dev), kw.to(dev), kw.to(dev), 1e-6, cos.to(dev), sin.to(dev), adjacent, k, v, ks, vs,
+                                torch.arange(T, device=dev), 0, nkv, d, torch.zeros(1, dtype=torch.int32, device=dev))
+    x = qkv[:, :nkv].double()
+    x = x / (x.square().mean(-1, keepdim=True) + torch.tensor(1e-6).double()).sqrt() * kw.double()
+    one, two = (slice(0, d, 2), slice(1, d, 2)) if adjacent else (slice(0, d // 2), slice(d // 2, d))
+    c, s = cos.double()[:, None], sin.double()[:, None]
+    want = torch.empty_like(x)
+    want[..., one], want[..., two] = x[..., one] * c - x[..., two] * s, x[..., one] * s + x[..., two] * c
+    want = want.float().to(torch.bfloat16).double()
+    got = ops.pages_8bit_to_bf16(k, v, ks, vs, torch.arange(T // page, dtype=torch.int32, device=dev))[0].cpu().double().transpose(1, 2).reshape(T, nkv, d)
+    for b in range(0, T, 16):
+        for h in range(nkv):
+            e = exponent(want[b:b + 16, h].abs().max().item(), dtype)
+            assert torch.equal(got[b:b + 16, h], encode(want[b:b + 16, h] * 2.0 ** -e, dtype) * 2.0 ** e), (b, h)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("norm,rot", [(False, False), (False, True), (True, True)])
+def test_write_keys_that_are_no_numbers(dtype, norm, rot):
+    """Not-a-number keys become zeros and infinite ones the largest number of their block's scale; rows beside them are not
+    touched by it (but share the scale).  A row with an infinity has no norm: all of it becomes zero."""
+    dev, ops = need_gpu(), _ops()
+    d, T = 64, 16
+    qkv = torch.randn(T, 2, d, generator=torch.Generator().manual_seed(4)).to(torch.bfloat16)
+    qkv[2, 0, 7] = float("nan")
+    qkv[3, 0, 8] = -float("inf")
+    qkv[4, 0] = 0
+    w = torch.ones(d, dtype=torch.bfloat16, device=dev) if norm else None
+    turn = torch.full((T, d // 2), 0.6, device=dev), torch.full((T, d // 2), 0.8, device=dev)
+    k, v, ks, vs = ops.cache_8bit_pools(1, 1, 16, d, dtype, dev)
+    ops.qk_norm_rope_write_8bit(qkv.view(T, -1).to(dev), w, w, 1e-6, turn[0] if rot else None, turn[1] if rot else None, True, k, v, ks, vs,
+                                torch.arange(T, device=dev), 0, 1, d, torch.zeros(1, dtype=torch.int32, device=dev))
+    top = 448.0 if dtype == torch.float8_e4m3fn else 127.0
+    got = (ops.pages_8bit_to_bf16(k, v, ks, vs, torch.zeros(1, dtype=torch.int32, device=dev))[0][0, 0].double() / ks.double().view(())).cpu()
+    assert torch.isfinite(got).all() and (got[4] == 0).all()
+    if norm:                                          # the sum of squares is no number, or infinite
+        assert (got[2] == 0).all() and (got[3, [i for i in range(d) if i not in (8, 9)]] == 0).all()
+        return
+    assert ks.item() == 2.0 ** 40
+    assert got[2, 7] == 0 and (got[2, 6] == 0 or not rot)
+    assert got[3, 8] == -top and (got[3, 9] == -top if rot else abs(got[3, 9]) < 1)
+
+
 def test_write_counts_slots_outside_the_pool():
     dev, ops = need_gpu(), _ops()
     pools = ops.cache_8bit_pools(3, 2, 16, 64, torch.int8, dev)
