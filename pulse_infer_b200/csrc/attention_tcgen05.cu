@@ -631,7 +631,8 @@ __global__ void __launch_bounds__(FA_MERGE_WARPS * 32) attn_prompt_merge_kernel(
     const int lane = threadIdx.x & 31;
     if (row >= rows) return;
     const int t = (int)(row / nq);
-    if (seg_len[token_seg[t]] == 1) return;          // single tokens are the decode kernel's
+    const int seg = token_seg[t];                    // -1: a row behind the last segment
+    if (seg < 0 || seg_len[seg] == 1) return;        // single tokens are the decode kernel's
     const float2* ml = reinterpret_cast<const float2*>(part_ml + (size_t)row * splits * 2);
     const float* acc = part_acc + (size_t)row * splits * D + E * lane;
     float mstar = -INFINITY;

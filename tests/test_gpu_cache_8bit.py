@@ -514,6 +514,58 @@ def test_a_step_of_portions_and_single_tokens(dtype, nq, nkv, d, page, window):
         t += n
 
 
+def test_a_step_recorded_and_replayed():
+    """Maps, page write, prompt (with shares of the keys) and decode attention in one CUDA graph: replayed over pages put back to
+    what they were, and again with other lengths and inputs in the same tensors, they give what the launched kernels give."""
+    dev, ops = need_gpu(), _ops()
+    nq, nkv, d, page, T = 8, 2, 128, 16, 60
+    segs = [(0, 3000, 40), (2, 77, 1), (1, 0, 18), (3, 500, 1)]
+    other = [(0, 2990, 38), (2, 79, 1), (1, 5, 18), (3, 498, 1)]                # what a replay meets; two rows are not used
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    table = torch.randperm(4 * 192, generator=torch.Generator().manual_seed(6)).int().view(4, 192).to(dev)
+    old = Pools(4 * 192, nkv, page, d, torch.int8, seed=5).on(dev)
+    old[2].fill_(2.0 ** -5); old[3].fill_(2.0 ** -6)
+    pools = [x.clone() for x in old]
+    slot, start, length = (i32([s[k] for s in segs]) for k in range(3))
+    qkv = torch.randn(T, (nq + 2 * nkv) * d, device=dev).to(torch.bfloat16)
+    err = torch.zeros(1, dtype=torch.int32, device=dev)
+    ws = ops.attention_decode_workspace(d, dev)
+    out = torch.zeros(T, nq * d, dtype=torch.bfloat16, device=dev)
+
+    def step():
+        out.zero_()
+        maps = ops.page_maps(table, slot, start, length, page, T, num_listed_pages=200, min_tokens=2)
+        q = ops.qk_norm_rope_write_8bit(qkv, None, None, 1e-6, None, None, True, *pools, maps.slot_map, nq, nkv, d, err)
+        ops.attention_prompt_8bit(q, nq * d, *pools, maps, start, length, [(3000, 40), (0, 18)], T, nq, nkv, d, None, d ** -0.5, out=out)
+        ops.attention_decode_8bit(q, nq * d, *pools, table, maps.seg_off, slot, start, length, T, 4, nq, nkv, d, None, d ** -0.5,
+                                  workspace=ws, out=out)
+
+    def back():
+        for x, y in zip(pools, old):
+            x.view(torch.uint8).copy_(y.view(torch.uint8))
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for now in (segs, other):
+        start.copy_(i32([s[1] for s in now])); length.copy_(i32([s[2] for s in now]))
+        qkv.copy_(torch.randn(T, (nq + 2 * nkv) * d, device=dev))
+        results = []
+        for run in (step, graph.replay, graph.replay):
+            back()
+            run()
+            torch.cuda.synchronize()
+            results.append([out.clone()] + [x.view(torch.uint8).clone() for x in pools])
+        used = sum(s[2] for s in now)
+        assert not (results[0][0][:used] == 0).all(1).any() and (results[0][0][used:] == 0).all()
+        for again in results[1:]:
+            assert all(torch.equal(x, y) for x, y in zip(results[0], again))
+    # the slot map is -1 behind the last token: two rows, counted once per key and value head in three of the calls
+    assert int(err.item()) == 3 * 2 * 2 * nkv and ops.attention_tcgen05_loaded_status() == 0
+
+
 @pytest.mark.parametrize("fit", [1, 90, 200, 333])
 @pytest.mark.parametrize("start", [0, 5000])
 def test_portions_with_more_tokens_than_rows(fit, start):
