@@ -272,7 +272,8 @@ def attention_prompt_8bit(q: torch.Tensor, q_stride: int, kcache: torch.Tensor, 
                           values: torch.Tensor | None = None) -> torch.Tensor:
     """Portions of prompts (segments of more than one token) over 8-bit pages: the pages that ``maps`` lists
     (``page_maps(..., min_tokens=2)`` with the same window) are expanded to bfloat16, exactly, and the tcgen05 prompt kernel
-    runs on the copies.  ``portions``: (start, length) of the segments of more than one token, on the host.  ``keys`` /
+    runs on the copies.  ``portions``: (start, length) of the segments of more than one token, on the host (a replayed recording of the
+    call may meet shorter ones, not longer ones).  ``keys`` /
     ``values``: bfloat16 [listed pages, kv heads, page size, d] for the copies, made here when missing; the layers of a step
     can share them.  Rows of single-token segments in ``out`` [num_tokens, nq d] are left as they are, and segments' tokens
     behind the first ``num_tokens`` are left out."""

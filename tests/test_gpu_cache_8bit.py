@@ -405,6 +405,28 @@ def test_decode_missing_pages_and_slots():
     assert (got[1:3] == 0).all() and torch.isfinite(got[3]).all() and (got[4:] == 9).all()
 
 
+@pytest.mark.parametrize("window", [None, 20])
+def test_decode_padded_with_segments_of_no_length(window):
+    """Segments without tokens in front, between and behind; their slots, starts and offsets may be anything."""
+    dev, ops = need_gpu(), _ops()
+    nq, nkv, d, page, lengths = 8, 2, 64, 16, [130, 1, 47]
+    seqs = Sequences(lengths, nkv, d, page, torch.int8, 3)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    q = torch.randn(5, nq * d, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+    out = torch.full((5, nq * d), 3.0, dtype=torch.bfloat16, device=dev)
+    pools, table = seqs.pools.on(dev), seqs.table.to(dev)
+    ops.attention_decode_8bit(q.to(dev), nq * d, *pools, table, i32(0, 0, 1, 1, 2, 3, -9), i32(99, 0, -1, 1, 2, 2 ** 31 - 1, 0),
+                              i32(7, lengths[0] - 1, -5, lengths[1] - 1, lengths[2] - 1, 2 ** 31 - 1, 0), i32(0, 1, 0, 1, 1, 0, 0), 5, 7, nq, nkv, d,
+                              window, 0.125, out=out)
+    got = out.cpu().double().view(5, nq, d)
+    for i, n in enumerate(lengths):
+        want, bound = attention_with_bound(q[i].double().view(nq, d), seqs.k[i], seqs.v[i], seqs.vs[i], n - 1, window, 0.125, F16_HALF_STEP, d)
+        assert ((got[i] - want).abs() <= bound).all()
+    assert (got[3:] == 3).all()
+    ops.attention_decode_8bit(q.to(dev), nq * d, *pools, table, i32(0), i32(0), i32(9), i32(0), 5, 1, nq, nkv, d, window, 0.125, out=out)
+    assert torch.equal(out.cpu().double().view(5, nq, d), got)                  # nothing to do at all
+
+
 def test_decode_is_the_same_in_a_graph_and_on_another_stream():
     dev, ops = need_gpu(), _ops()
     seqs = Sequences([700, 65, 2000], 2, 128, 16, torch.float8_e4m3fn)
