@@ -31,7 +31,8 @@
 // to the first byte (lengths, block table, pages: three round trips) and 5 the sums between warps and CTAs at the end; one of
 // 32,768 keys, int8: 23.4 us.  Tried: operands through a queue in shared memory of each warp, by bulk copies with an mbarrier per
 // 4 KB (83, 22.7 and 25.4 us; also with 12 warps) or by cp.async (slower still); spans of whole CTAs, a barrier at each piece
-// (113, 25.8 and 31.7 us).
+// (113, 25.8 and 31.7 us); shares counted in blocks of 16 keys instead of tiles of 64 (evener, but more cuts and tiles that are
+// not full: 85.2, 21.7 and 24.3 us).
 #include <math.h>
 
 #include "cache_8bit.cuh"
