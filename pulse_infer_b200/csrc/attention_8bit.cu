@@ -27,9 +27,10 @@
 // A group of more than eight query heads is cut in pieces of eight, and its keys are read once for each (from L2 mostly).
 //
 // Measured (B200, 8 kv heads of 128; device time of a launch among others): 64 requests of 130 to 8,190 keys, 40 query heads,
-// e4m3: 85 us, 459 MB at 5.4 TB/s (6.9 in the middle); 8 requests of 4,096 keys: 21.4 us, of which 10 are transfer, 3 to 4 the way
-// to the first byte (lengths, block table, pages: three round trips) and 5 the sums between warps and CTAs at the end; one of
-// 32,768 keys, int8: 23.4 us.  Tried: operands through a queue in shared memory of each warp, by bulk copies with an mbarrier per
+// e4m3: 85 us, 459 MB at 5.4 TB/s (6.9 in the middle); 8 requests of 4,096 keys: 21.4 us for
+// 10.2 us of transfer: the first tiles are asked for after 2.5 to 4.5 us (lengths, block table), by all SMs at once, and are
+// there after 6.5 to 9; a warp has three or four tiles and is done after 8 to 19; the sums between warps and CTAs take 3.  One
+// request of 32,768 keys, int8: 23.4 us.  Tried: operands through a queue in shared memory of each warp, by bulk copies with an mbarrier per
 // 4 KB (83, 22.7 and 25.4 us; also with 12 warps) or by cp.async (slower still); spans of whole CTAs, a barrier at each piece
 // (113, 25.8 and 31.7 us); shares counted in blocks of 16 keys instead of tiles of 64 (evener, but more cuts and tiles that are
 // not full: 85.2, 21.7 and 24.3 us).
