@@ -544,8 +544,8 @@ def test_a_step_recorded_and_replayed():
     segs = [(0, 3000, 40), (2, 77, 1), (1, 0, 18), (3, 500, 1)]
     other = [(0, 2990, 38), (2, 79, 1), (1, 5, 18), (3, 498, 1)]                # what a replay meets; two rows are not used
     i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
-    table = torch.randperm(4 * 192, generator=torch.Generator().manual_seed(6)).int().view(4, 192).to(dev)
-    old = Pools(4 * 192, nkv, page, d, torch.int8, seed=5).on(dev)
+    table = torch.randperm(4 * 200, generator=torch.Generator().manual_seed(6)).int().view(4, 200).to(dev)
+    old = Pools(4 * 200, nkv, page, d, torch.int8, seed=5).on(dev)
     old[2].fill_(2.0 ** -5); old[3].fill_(2.0 ** -6)
     pools = [x.clone() for x in old]
     slot, start, length = (i32([s[k] for s in segs]) for k in range(3))
