@@ -486,7 +486,8 @@ PI_EXPORT int pi_logit_rules(const RuleArgs* args, cudaStream_t stream) {
     if (vocab <= 0 || ld < vocab || out_ld < vocab) return pi_refuse("pi_logit_rules: vocab=%d ld=%lld out_ld=%lld", vocab, ld, out_ld);
     if (rows > 65535) return pi_refuse("pi_logit_rules: %d rows are beyond the grid limit", rows);
     if (vocab > 2147483647 - RULE_SLICE) return pi_refuse("pi_logit_rules: vocab=%d is beyond the limit", vocab);
-    if (history_total > (1 << 30) || bias_total > (1 << 30)) return pi_refuse("pi_logit_rules: histories of %lld or %lld biases are beyond the limit", history_total, bias_total);
+    // a count of an id stays below bit 30 of its mark
+    if (history_total >= (1 << 30) || bias_total > (1 << 30)) return pi_refuse("pi_logit_rules: histories of %lld or %lld biases are beyond the limit", history_total, bias_total);
     RuleParams p;
     p.logits = logits; p.ld = ld; p.out = out; p.out_ld = out_ld; p.vocab = vocab;
     p.vec = (ld % 4 == 0 && out_ld % 4 == 0 && (((uintptr_t)logits | (uintptr_t)out) & 15) == 0) ? 1 : 0;

@@ -24,3 +24,17 @@ def test_formats_that_do_not_exist(bad):
     from pulse_infer_b200 import ops
     with pytest.raises(ops.KernelError):
         ops.cache_8bit_pools(*bad, "cpu")
+
+
+def test_histories_beyond_the_counter_are_refused():
+    """2^30 entries of one id would carry its count into the bit that says that the id has a bias.  (The launcher refuses
+    before it looks at a pointer or at the device.)"""
+    import ctypes
+    from pulse_infer_b200.ops import kernels
+    lib = kernels._lib("sampling")
+    launch = lib.pi_logit_rules
+    launch.argtypes = kernels._LOGIT_RULES.argtypes
+    for history, biases in ((1 << 30, 0), ((1 << 30) + 1, 0), (1 << 40, 0), (0, (1 << 30) + 1)):
+        record = kernels._LOGIT_RULES.pack(0, 8, 0, 8, 1, 8, 0, 0, history, 0, 0, 0, 0, 0, 0, 0, biases, 0, 0, 0)
+        assert launch(record, None) == -1, (history, biases)
+        assert b"beyond the limit" in lib.pi_last_error()
