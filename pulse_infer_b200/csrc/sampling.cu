@@ -10,6 +10,7 @@
 //   top-p        demo/qwen3_infer.cpp:395-409   shortest prefix (by descending logit) with cumulative mass >= p
 //   draw         demo/qwen3_infer.cpp:411-422   uniform in [0, total), first candidate with cumulative >= draw
 //   penalty/ban  demo/qwen3_infer.cpp:251-264, 522-535
+// A row in which no token is left - every logit is -inf, by rules, or NaN - gives -1, which ends a request.
 // Differences by design: the draw comes from a counter-based generator keyed by (seed, draw index) so a
 // request's tokens do not depend on batching; the cumulative walk is in index order rather than sorted
 // order (the distribution is the same); all logits equal to the top-p threshold are kept.
@@ -46,11 +47,12 @@ __device__ __forceinline__ ArgMax better(ArgMax a, ArgMax b) {
     return a;
 }
 
+// index -1 where there is nothing to choose: a logit of -inf is a forbidden token, NaN is none
 __device__ ArgMax block_argmax(const float* __restrict__ x, int n, ArgMax* sh /* 33 */) {
     ArgMax best = {-INFINITY, -1};
     for (int i = threadIdx.x; i < n; i += blockDim.x) {
         const float v = x[i];
-        if (v == v && (best.i < 0 || v > best.v)) { best.v = v; best.i = i; }
+        if (v > best.v) { best.v = v; best.i = i; }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -197,7 +199,7 @@ __global__ void sample_kernel(const float* __restrict__ logits, int ld, int voca
     const int entry = row_entry != nullptr ? (int)row_entry[2 * row] : row;
     const unsigned long long counter = row_entry != nullptr ? (unsigned long long)row_entry[2 * row + 1] : counters[row];
     const float temp = temperature[entry];
-    if (temp <= 0.0f || top.i < 0) {
+    if (temp <= 0.0f || top.i < 0 || top.v == INFINITY) {      // +inf has all of the probability
         if (threadIdx.x == 0) out[row] = top.i;
         return;
     }

@@ -772,7 +772,7 @@ def linear(x, weight: torch.Tensor, out_dtype: torch.dtype | None = None, residu
 
 # ---- sampling ---------------------------------------------------------------------------------------------------------
 def argmax(logits: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
-    """logits fp32 [n, V] -> int32 [n]; the lowest index wins ties."""
+    """logits fp32 [n, V] -> int32 [n]; the lowest index wins ties.  -1 for a row without a number above -inf."""
     _need_cuda(logits)
     if logits.dtype != torch.float32 or logits.stride(-1) != 1:
         raise KernelError("logits must be float32 with unit stride")
@@ -790,7 +790,8 @@ def argmax(logits: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tenso
 def sample(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor, top_p: torch.Tensor,
            seeds: torch.Tensor, counters: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
     """Per-row temperature / top-k / top-p sampling; temperature <= 0 means greedy for that row.
-    seeds and counters are int64 (read as unsigned); the uniform draw depends on them only."""
+    seeds and counters are int64 (read as unsigned); the uniform draw depends on them only.  As ``argmax``, -1 for a row
+    without a number above -inf; a logit of +inf is chosen."""
     _need_cuda(logits, temperature, top_k, top_p, seeds, counters)
     n, V = logits.shape
     if logits.dtype != torch.float32 or logits.stride(-1) != 1:

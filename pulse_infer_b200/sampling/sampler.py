@@ -75,7 +75,7 @@ class Sampler:
                prompt_lens: list | None = None) -> list:
         """logits float32 [n, V]; params[i] SamplingParams; draw_index[i] how many tokens request i has
         drawn so far; history[i] the tokens that penalties and grammars look at (ids, a list or an int32 array), its first
-        prompt_lens[i] (default: none) the prompt.  Returns n token ids."""
+        prompt_lens[i] (default: none) the prompt.  Returns n token ids; -1 where the rules leave no token."""
         out = self.sample_device(logits, params, draw_index, history, prompt_lens)
         return [] if out is None else out.tolist()
 
