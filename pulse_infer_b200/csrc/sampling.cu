@@ -26,6 +26,8 @@ __device__ __forceinline__ unsigned ordered_key(float f) {
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
+#define KEY_MINUS_INF 0x007fffffu      // ordered_key(-INFINITY)
+
 __device__ __forceinline__ unsigned long long splitmix64(unsigned long long z) {
     z += 0x9E3779B97F4A7C15ull;
     z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
@@ -236,8 +238,9 @@ __global__ void sample_kernel(const float* __restrict__ logits, int ld, int voca
         tie_cut = sh_pick;
         __syncthreads();
     }
-    // key 0 is NaN only; with no top-k, key_k stays 0 and every number is kept
-    auto kept_k = [&](int i, unsigned key) { return key != 0u && (key > key_k || (key == key_k && i <= tie_cut)); };
+    // NaN and -inf (a forbidden token) are never kept: a weight of zero could be drawn, by a draw of exactly zero or where the
+    // sums round; with no top-k, key_k stays 0 and every other number is kept
+    auto kept_k = [&](int i, unsigned key) { return key > KEY_MINUS_INF && (key > key_k || (key == key_k && i <= tie_cut)); };
     const float inv_t = 1.0f / temp;
 
     // ---- top-p: the largest value v whose upper mass (logit >= v, inside the top-k set) reaches p * Z ---

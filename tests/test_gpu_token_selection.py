@@ -95,3 +95,22 @@ def test_a_request_without_a_choice_ends_and_the_others_go_on(model_folders):
             assert len(out) == 4 and out[3] == -1 and min(out[:3]) >= 0
         assert engine.get_result(c) == alone and engine.get_request(c).finish_reason == "length"
         assert list(engine.get_stats().free_pages) == [40]
+
+
+@pytest.mark.parametrize("vocab", [31, 515, 40000])
+@pytest.mark.parametrize("temp,k,p", [(1.0, 0, 0.0), (0.7, 12, 0.0), (1.0, 0, 0.99), (1.3, 20, 0.9)])
+def test_a_forbidden_token_is_never_drawn(vocab, temp, k, p):
+    """The draw of (seed 0, counter 345377) is exactly zero, which the first kept token's cumulative weight reaches even if
+    it is zero: tokens of logit -inf must not be kept.  Others: whatever the draw and however few are allowed."""
+    import plain_model
+    dev, ops = need_gpu(), _ops()
+    assert plain_model.uniform_from(0, 345377) == 0.0
+    g = torch.Generator().manual_seed(vocab)
+    row = torch.randn(vocab, generator=g)
+    allowed = torch.randperm(vocab - 8, generator=g)[:7] + 4                     # fewer than top-k asks for; not the first, nor the last
+    masked = torch.full((vocab,), -INF)
+    masked[allowed] = row[allowed]
+    counters = [345377] + list(range(200))
+    got = _sample(ops, dev, masked.repeat(len(counters), 1), temp, k, p, seed=0, counters=counters)
+    assert set(got) <= set(allowed.tolist())
+    assert p or k or got[0] == int(allowed.min())
