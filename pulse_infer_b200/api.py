@@ -54,10 +54,9 @@ class Engine:
                     ignore_eos: bool = False, repetition_penalty: float = 1.0, frequency_penalty: float = 0.0,
                     logit_bias=(), grammar=None) -> int:
         """``logit_bias``: {token: value} or (token, value) pairs.  For the other options see ``SamplingParams``."""
-        bias = tuple(logit_bias.items()) if hasattr(logit_bias, "items") else tuple(tuple(b) for b in logit_bias)
         params = SamplingParams(temperature=temperature, top_k=top_k, top_p=top_p, presence_penalty=presence_penalty,
                                 banned_tokens=tuple(banned_tokens), seed=seed, repetition_penalty=repetition_penalty,
-                                frequency_penalty=frequency_penalty, logit_bias=bias, grammar=grammar)
+                                frequency_penalty=frequency_penalty, logit_bias=logit_bias, grammar=grammar)
         return self.engine.add_request(list(prompt_tokens), max_new_tokens, params, ignore_eos)
 
     def step(self) -> list:

@@ -6,6 +6,8 @@ from __future__ import annotations
 import math
 from dataclasses import dataclass
 
+F32_MAX, F32_TINY = (2.0 - 2.0 ** -23) * 2.0 ** 127, 2.0 ** -126       # largest and smallest normal number of 32 bits
+
 
 @dataclass(frozen=True)
 class SamplingParams:
@@ -19,16 +21,28 @@ class SamplingParams:
     # in the order in which they apply (ops.logit_rules): repetition, frequency, presence, biases and bans, grammar
     repetition_penalty: float = 1.0  # logits of tokens in prompt or output are divided by it if positive, else multiplied
     frequency_penalty: float = 0.0   # subtracted once for every time a token was generated
-    logit_bias: tuple = ()           # (token, value) pairs that are added
+    logit_bias: tuple = ()           # (token, value) pairs, or {token: value}, that are added; -inf forbids the token
     # an object with ``token_mask(generated) -> None or ceil(vocabulary / 32) 32-bit words`` (bit v % 32 of word v / 32 set:
     # token v is allowed), asked before every token with the tokens generated so far
     grammar: object = None
 
     def __post_init__(self):
-        if not (self.repetition_penalty > 0.0 and math.isfinite(self.repetition_penalty)):
-            raise ValueError(f"repetition_penalty must be positive and finite, got {self.repetition_penalty}")
-        if not math.isfinite(self.frequency_penalty):
-            raise ValueError(f"frequency_penalty must be finite, got {self.frequency_penalty}")
+        # what the kernel cannot take is refused here: in a step it would stop the other requests too
+        if not F32_TINY <= self.repetition_penalty <= F32_MAX:
+            raise ValueError(f"repetition_penalty must be positive and finite in 32 bits, got {self.repetition_penalty}")
+        if not abs(self.frequency_penalty) <= F32_MAX:
+            raise ValueError(f"frequency_penalty must be finite in 32 bits, got {self.frequency_penalty}")
+        try:
+            pairs = self.logit_bias.items() if hasattr(self.logit_bias, "items") else self.logit_bias
+            bias = tuple((int(t), float(v)) for t, v in pairs)
+            banned = tuple(int(t) for t in self.banned_tokens)
+        except (TypeError, ValueError, OverflowError) as exc:
+            raise ValueError(f"logit_bias must hold (token, value) pairs and banned_tokens token ids: {exc}") from exc
+        for token, value in bias:
+            if not (abs(value) <= F32_MAX or value == -math.inf):
+                raise ValueError(f"logit_bias of token {token} must be finite in 32 bits or -inf, got {value}")
+        object.__setattr__(self, "logit_bias", bias)
+        object.__setattr__(self, "banned_tokens", banned)
         if self.grammar is not None and not callable(getattr(self.grammar, "token_mask", None)):
             raise ValueError("a grammar needs a token_mask(generated) method")
 

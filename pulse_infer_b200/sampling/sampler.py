@@ -88,9 +88,9 @@ class Sampler:
         prompts = [min(int(prompt_lens[i]), tokens[i].size) if prompt_lens is not None else 0 for i in range(n)]
         biases = []
         for p in params:
-            row = {int(t): float(v) for t, v in p.logit_bias}
-            row.update((int(t), float("-inf")) for t in p.banned_tokens)
-            biases.append(row)
+            row = dict(p.logit_bias)
+            row.update((t, float("-inf")) for t in p.banned_tokens)
+            biases.append({t: v for t, v in row.items() if 0 <= t < V})     # ids that are none may be beyond 32 bits
         words = (V + 31) // 32
         masks, mask_row = [], [-1] * n
         for i, p in enumerate(params):

@@ -262,3 +262,16 @@ def test_logit_rules_output_that_overlaps_the_logits():
     for a, b in (((0, 80), (0, 80)), ((0, 200), (70, 200)), ((100, 200), (30, 200)), ((0, 70), (210, 70)), ((300, 80), (60, 80))):
         want = view(*a).clone()
         assert torch.equal(ops.logit_rules(view(*a), *rules, out=view(*b)), want)
+
+
+def test_ids_that_no_vocabulary_has_are_passed_over():
+    """Through the sampler, also where 32 bits do not hold them."""
+    from pulse_infer_b200.sampling import Sampler, SamplingParams
+    dev = need_gpu()
+    V = 300
+    x = torch.randn(2, V, generator=torch.Generator().manual_seed(1))
+    best = int(x[0].argmax())
+    odd = (2 ** 40, -1, -2 ** 40, V, 2 ** 31, -2 ** 31 - 1, 2 ** 32 + best)
+    got = Sampler(dev).sample(x.to(dev), [SamplingParams(banned_tokens=odd, logit_bias=tuple((t, 50.0) for t in odd)),
+                                          SamplingParams(banned_tokens=odd + (int(x[1].argmax()),))], [0, 0])
+    assert got == [best, int(x[1].topk(2).indices[1])]

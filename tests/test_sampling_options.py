@@ -42,3 +42,21 @@ def test_token_array_follows_the_request():
     req.preempt()
     req.add_sampled_token(9, ())
     assert req.token_array().tolist() == req.all_tokens() and req.token_array().dtype == np.int32
+
+
+@pytest.mark.parametrize("kw", [dict(logit_bias=((3, float("nan")),)), dict(logit_bias=((3, float("inf")),)), dict(logit_bias=((3, 1e39),)),
+                                dict(logit_bias=((3, -1e39),)), dict(logit_bias=(3,)), dict(logit_bias=(("a", 1.0),)), dict(logit_bias=((3, None),)),
+                                dict(banned_tokens=("a",)), dict(banned_tokens=(None,)), dict(logit_bias=((3, 1.0, 2.0),)), dict(logit_bias=7),
+                                dict(repetition_penalty=1e39), dict(repetition_penalty=1e-50), dict(repetition_penalty=1e-39),
+                                dict(frequency_penalty=1e39), dict(frequency_penalty=-1e39)])
+def test_rules_that_32_bits_cannot_hold_or_that_are_no_rules_are_refused(kw):
+    """When the options are made, not in the middle of a step that other requests share."""
+    with pytest.raises(ValueError):
+        SamplingParams(**kw)
+
+
+def test_rules_that_are_taken():
+    p = SamplingParams(logit_bias={7: 1, np.int64(8): -float("inf")}, banned_tokens=[np.int32(4), 2 ** 40, -1])
+    assert p.logit_bias == ((7, 1.0), (8, -float("inf"))) and p.banned_tokens == (4, 2 ** 40, -1)
+    assert SamplingParams(logit_bias=[[5, 2.0], (6, 3e38)]).logit_bias == ((5, 2.0), (6, 3e38))
+    assert SamplingParams(presence_penalty=float("inf")).needs_history
