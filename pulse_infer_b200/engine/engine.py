@@ -15,6 +15,7 @@ step before in that mode; results, finish reasons and the order of tokens per re
 """
 from __future__ import annotations
 
+import warnings
 from dataclasses import dataclass, field
 
 from ..sampling.params import SamplingParams
@@ -39,7 +40,8 @@ class ContinuousBatchEngine:
                  max_tokens_per_step: int | None = None, max_sequences: int | None = None, lookahead: bool = False):
         """``runner``: the step function (``open``/``close`` happen through its cache manager);
         ``sampler``: ``sample(logits, params, draw_index, history) -> token ids``; also with ``prompt_lens=`` when a
-        request's options tell its prompt from its output (``SamplingParams.needs_prompt_len``).
+        request's options tell its prompt from its output (``SamplingParams.needs_prompt_len``), and with ``allowed=``,
+        the masks of the requests' grammars, when one has a grammar.
         ``lookahead`` needs ``sampler.sample_device`` and ``runner.step(..., tokens_from=)``."""
         self.runner = runner
         self.sampler = sampler
@@ -117,14 +119,26 @@ class ContinuousBatchEngine:
 
     def _launch(self, batch: ScheduledBatch, tokens_from=None) -> _Launched | None:
         entries = [(req, n) for req, n in batch.entries if not req.is_finished()]     # ended by the read-back just before
-        segments, sampling_reqs = [], []
+        segments, sampling_reqs, allowed, ran = [], [], [], []
         for req, n in entries:
             tokens = req.get_next_chunk_tokens(n)
             all_in = req.num_computed_tokens + n == req.total_input_tokens()
             wants = all_in and req.can_generate_more()
+            if wants and req.sampling.grammar is not None:
+                # asked before the step: one that fails ends its own request, not the step that others share
+                try:
+                    allowed.append(req.sampling.token_mask(list(req.generated_tokens), self.runner.vocab_size))
+                except Exception as exc:
+                    warnings.warn(f"request {req.request_id} ends: its grammar failed: {exc!r}")
+                    self.scheduler.abort(req.request_id, "grammar_error")
+                    continue
+            elif wants:
+                allowed.append(None)
+            ran.append((req, n))
             segments.append(Segment(req.request_id, tokens, [n - 1] if wants else []))
             if wants:
                 sampling_reqs.append(req)
+        entries = ran
         rec = _Launched(batch, entries)
         if not segments:
             return rec
@@ -142,6 +156,8 @@ class ContinuousBatchEngine:
                 history = [r.token_array() if r.sampling.needs_history else () for r in sampling_reqs]
                 if any(r.sampling.needs_prompt_len for r in sampling_reqs):
                     more = {"prompt_lens": [r.prompt_len() for r in sampling_reqs]}
+                if any(r.sampling.grammar is not None for r in sampling_reqs):
+                    more["allowed"] = allowed
             params = [r.sampling for r in sampling_reqs]
             draws = [r.num_generated() for r in sampling_reqs]
             rec.sampling_reqs = sampling_reqs

@@ -6,6 +6,8 @@ from __future__ import annotations
 import math
 from dataclasses import dataclass
 
+import numpy as np
+
 F32_MAX, F32_TINY = (2.0 - 2.0 ** -23) * 2.0 ** 127, 2.0 ** -126       # largest and smallest normal number of 32 bits
 
 
@@ -45,6 +47,18 @@ class SamplingParams:
         object.__setattr__(self, "banned_tokens", banned)
         if self.grammar is not None and not callable(getattr(self.grammar, "token_mask", None)):
             raise ValueError("a grammar needs a token_mask(generated) method")
+
+    def token_mask(self, generated: list, vocab_size: int):
+        """What the grammar allows behind ``generated``: ceil(vocab_size / 32) 32-bit words, or None for everything."""
+        if self.grammar is None:
+            return None
+        mask = self.grammar.token_mask(generated)
+        if mask is None:
+            return None
+        mask, words = np.ascontiguousarray(mask).reshape(-1), (vocab_size + 31) // 32
+        if mask.size != words or mask.dtype.itemsize != 4 or mask.dtype.kind not in "iu":
+            raise ValueError(f"a token mask must hold {words} 32-bit words, got {mask.size} of {mask.dtype}")
+        return mask.view(np.int32)
 
     @property
     def greedy(self) -> bool:

@@ -72,14 +72,16 @@ class Sampler:
         return dev
 
     def sample(self, logits: torch.Tensor, params: list, draw_index: list, history: list | None = None,
-               prompt_lens: list | None = None) -> list:
+               prompt_lens: list | None = None, allowed: list | None = None) -> list:
         """logits float32 [n, V]; params[i] SamplingParams; draw_index[i] how many tokens request i has
         drawn so far; history[i] the tokens that penalties and grammars look at (ids, a list or an int32 array), its first
-        prompt_lens[i] (default: none) the prompt.  Returns n token ids; -1 where the rules leave no token."""
-        out = self.sample_device(logits, params, draw_index, history, prompt_lens)
+        prompt_lens[i] (default: none) the prompt; allowed[i] what request i's grammar allows (``SamplingParams.token_mask``;
+        asked for here if ``allowed`` is not given).  Returns n token ids; -1 where the rules leave no token."""
+        out = self.sample_device(logits, params, draw_index, history, prompt_lens, allowed)
         return [] if out is None else out.tolist()
 
-    def _apply_rules(self, logits: torch.Tensor, params: list, history: list | None, prompt_lens: list | None) -> torch.Tensor:
+    def _apply_rules(self, logits: torch.Tensor, params: list, history: list | None, prompt_lens: list | None,
+                     allowed: list | None) -> torch.Tensor:
         """``logits`` after the rules of every row, in a new tensor."""
         n, V = logits.shape
         told = history is not None
@@ -91,16 +93,11 @@ class Sampler:
             row = dict(p.logit_bias)
             row.update((t, float("-inf")) for t in p.banned_tokens)
             biases.append({t: v for t, v in row.items() if 0 <= t < V})     # ids that are none may be beyond 32 bits
-        words = (V + 31) // 32
-        masks, mask_row = [], [-1] * n
-        for i, p in enumerate(params):
-            mask = p.grammar.token_mask(tokens[i][prompts[i]:].tolist()) if p.grammar is not None else None
-            if mask is not None:
-                mask = np.ascontiguousarray(mask).reshape(-1)
-                if mask.size != words or mask.dtype.itemsize != 4 or mask.dtype.kind not in "iu":
-                    raise ValueError(f"a token mask must hold {words} 32-bit words, got {mask.size} of {mask.dtype}")
-                mask_row[i] = len(masks)
-                masks.append(mask.view(np.int32))
+        if allowed is None:
+            allowed = [p.token_mask(tokens[i][prompts[i]:].tolist(), V) for i, p in enumerate(params)]
+        masks = [m for m in allowed if m is not None]
+        ends = np.cumsum([m is not None for m in allowed])
+        mask_row = [int(end) - 1 if m is not None else -1 for m, end in zip(allowed, ends)]
         f32 = lambda v: np.asarray(v, dtype=np.float32).view(np.int32)  # noqa: E731
         off = lambda v: np.concatenate([[0], np.cumsum(v)]).astype(np.int32)  # noqa: E731
         with_history = [p.needs_history and told for p in params]
@@ -121,18 +118,18 @@ class Sampler:
         if bias_tokens.numel():
             kw.update(bias_off=bias_off, bias_tokens=bias_tokens, bias_values=as_f32(bias_values))
         if masks:
-            kw.update(mask=mask.view(len(masks), words), mask_row=rows)
+            kw.update(mask=mask.view(len(masks), -1), mask_row=rows)
         return ops.logit_rules(logits, flat, history_off, prompt_len, as_f32(repetition), as_f32(frequency), as_f32(presence), **kw)
 
     def sample_device(self, logits: torch.Tensor, params: list, draw_index: list, history: list | None = None,
-                      prompt_lens: list | None = None):
+                      prompt_lens: list | None = None, allowed: list | None = None):
         """The same, but the token ids stay on the device (int32 [n], or None for no rows): the caller reads them
         when it needs them, and the next step can take them as its input without a round trip."""
         n = logits.shape[0]
         if n == 0:
             return None
         if any(p.edits_logits for p in params):
-            logits = self._apply_rules(logits, params, history, prompt_lens)
+            logits = self._apply_rules(logits, params, history, prompt_lens, allowed)
         if all(p.greedy for p in params):
             return ops.argmax(logits)
         self._ensure_tables()

@@ -275,3 +275,42 @@ def test_ids_that_no_vocabulary_has_are_passed_over():
     got = Sampler(dev).sample(x.to(dev), [SamplingParams(banned_tokens=odd, logit_bias=tuple((t, 50.0) for t in odd)),
                                           SamplingParams(banned_tokens=odd + (int(x[1].argmax()),))], [0, 0])
     assert got == [best, int(x[1].topk(2).indices[1])]
+
+
+@pytest.mark.parametrize("lookahead", [False, True])
+def test_a_grammar_that_fails_ends_its_own_request_only(model_folders, lookahead):
+    """One that raises, one whose mask has another size, one whose mask is of another type: each ends its request with what it
+    generated so far; the others, and a later request, get what they get alone."""
+    import warnings
+    from pulse_infer_b200 import Engine
+    from tiny_configs import CONFIGS
+    need_gpu()
+    V = CONFIGS["A"].vocab_size
+
+    class Fails(_Grammar):
+        def __init__(self, how, after):
+            super().__init__(V)
+            self.how, self.after = how, after
+
+        def token_mask(self, generated):
+            mask = super().token_mask(generated)
+            return mask if len(generated) < self.after else self.how()
+
+    def raises():
+        raise RuntimeError("no such state")
+
+    engine = Engine(model_folders["A"], dtype="float32", page_size=8, num_pages=60, max_batch_size=6, lookahead=lookahead)
+    alone = engine.generate([[4, 5]], 7, ignore_eos=True)[0]
+    ids = [engine.add_request([1, 2, 3], 6, ignore_eos=True, grammar=Fails(how, after))
+           for how, after in ((raises, 2), (lambda: np.zeros(3, np.int32), 0), (lambda: np.zeros((V + 31) // 32, np.int64), 1), (lambda: "no", 3))]
+    free = engine.add_request([4, 5], 7, ignore_eos=True)
+    good = engine.add_request([1, 2, 3], 6, ignore_eos=True, grammar=_Grammar(V))
+    with warnings.catch_warnings(record=True) as told:
+        warnings.simplefilter("always")
+        engine.run_until_complete()
+    assert [len(engine.get_result(i)) for i in ids] == [2, 0, 1, 3]
+    assert [engine.get_request(i).finish_reason for i in ids] == ["grammar_error"] * 4
+    assert sum("grammar" in str(w.message) for w in told) == 4 and any("no such state" in str(w.message) for w in told)
+    assert engine.get_result(free) == alone and len(engine.get_result(good)) == 6
+    assert [t % 7 for t in engine.get_result(good)[:4]] == [0, 1, 2, 3]
+    assert engine.generate([[4, 5]], 7, ignore_eos=True)[0] == alone and list(engine.get_stats().free_pages) == [60]
