@@ -55,7 +55,7 @@ class SamplingParams:
         mask = self.grammar.token_mask(generated)
         if mask is None:
             return None
-        mask, words = np.ascontiguousarray(mask).reshape(-1), (vocab_size + 31) // 32
+        mask, words = np.array(mask).reshape(-1), (vocab_size + 31) // 32       # a copy: the grammar may fill its array again
         if mask.size != words or mask.dtype.itemsize != 4 or mask.dtype.kind not in "iu":
             raise ValueError(f"a token mask must hold {words} 32-bit words, got {mask.size} of {mask.dtype}")
         return mask.view(np.int32)

@@ -60,3 +60,16 @@ def test_rules_that_are_taken():
     assert p.logit_bias == ((7, 1.0), (8, -float("inf"))) and p.banned_tokens == (4, 2 ** 40, -1)
     assert SamplingParams(logit_bias=[[5, 2.0], (6, 3e38)]).logit_bias == ((5, 2.0), (6, 3e38))
     assert SamplingParams(presence_penalty=float("inf")).needs_history
+
+
+def test_a_grammar_may_fill_the_same_array_every_time():
+    class Shared:
+        words = np.zeros(3, dtype=np.int32)
+
+        def token_mask(self, generated):
+            self.words[:] = len(generated)
+            return self.words
+
+    p = SamplingParams(grammar=Shared())
+    masks = [p.token_mask([0] * n, 96) for n in (1, 2, 3)]
+    assert [m.tolist() for m in masks] == [[n] * 3 for n in (1, 2, 3)]
