@@ -48,6 +48,7 @@
 #define FA_ROWS 256          // rows of a CTA: two query tiles
 #define FA_BN 128            // keys of a tile
 #define FA_STAGES 5          // ring of K / V tiles
+#define FA_NOTES 4           // ring of notes of missing keys; three are in use at a time
 #define FA_THREADS 320
 #define FA_SPIN_LIMIT (1u << 22)
 
@@ -56,6 +57,9 @@ __device__ unsigned g_fa_status;
 struct FaParams {
     const bf16* q; int q_stride;
     const int* block_table; int bt_stride;
+    // pages that are copies: place i < copies holds a copy of page listed[i] of a pool of listed_pages, and is missing if that
+    // is not there.  Null: the pages are the pool's.
+    const int* listed; long long listed_pages; long long copies;
     const int* seg_off; const int* seg_slot; const int* seg_start; const int* seg_len;
     bf16* out;
     int nq, nkv, group;
@@ -225,6 +229,13 @@ __device__ __forceinline__ void fa_row_mask(float (&v)[FA_BN], int k0, int pos_r
         if (i > hi || i < lo) v[i] = -INFINITY;
 }
 
+// keys without a page: bit i of `missing` is keys 8 i .. 8 i + 7
+__device__ __forceinline__ void fa_row_drop(float (&v)[FA_BN], unsigned missing) {
+#pragma unroll
+    for (int i = 0; i < FA_BN; ++i)
+        if (missing & (1u << (i / 8))) v[i] = -INFINITY;
+}
+
 __device__ __forceinline__ float fa_row_max(const float (&v)[FA_BN]) {
     float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
 #pragma unroll
@@ -343,11 +354,14 @@ attn_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     unsigned long long* s_full = bars + 2 * FA_STAGES;    // [2] MMA -> softmax of query tile x: scores are in TMEM
     unsigned long long* p_ready = s_full + 2;             // [2] softmax (4 warps) -> MMA: P written, O rescaled, S read
     unsigned long long* pv_done = s_full + 4;             // [2] MMA -> softmax: the last product with the values is done
-    unsigned* tmem_slot = reinterpret_cast<unsigned*>(s_full + 6);
+    unsigned long long* noted = s_full + 6;               // [FA_NOTES] TMA warp -> softmax: the tile's missing keys are noted
+    unsigned* tmem_slot = reinterpret_cast<unsigned*>(noted + FA_NOTES);
     volatile unsigned* failed = tmem_slot + 1;
+    volatile unsigned* missing_keys = tmem_slot + 2;      // [FA_NOTES] eight keys to a bit
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
+        for (int i = 0; i < FA_NOTES; ++i) fa_mbar_init(&noted[i], 1);
         for (int i = 0; i < FA_STAGES; ++i) { fa_mbar_init(&full[i], 1); fa_mbar_init(&empty[i], 1); }
         for (int i = 0; i < 2; ++i) { fa_mbar_init(&s_full[i], 1); fa_mbar_init(&p_ready[i], 4); fa_mbar_init(&pv_done[i], 1); }
         *failed = 0;
@@ -405,9 +419,12 @@ attn_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             const int key = kbegin + j * FA_BN + lane * ps;
             return (j < num_tiles && lane < pages_per_tile && key < kend && key / ps < p.bt_stride) ? table[key / ps] : -1;
         };
+        const int first_seen = fa_window_lo(pos_first, p.window);
         int page = lookup(0);
         for (int j = 0; j < num_tiles && !*failed; ++j) {
             const int next_page = lookup(j + 1);
+            int source = 0;                                // needed below, when the loads are on their way
+            if (p.listed != nullptr) source = page >= 0 && page < p.copies ? p.listed[page] : -1;
             const unsigned mask = __ballot_sync(0xffffffffu, page >= 0);
             const unsigned bytes = (unsigned)__popc(mask) * page_bytes * HALVES;
             const int row = (page * p.nkv + kvh) * ps;
@@ -425,6 +442,17 @@ attn_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                 }
             }
             if (!ok) break;
+            // A page that some query of the block should see and that is not there: its keys are left out of the softmax, whatever
+            // the ring holds in their place.  (A slot of the notes is free again: V(j) was asked for, so the scores of tile j - 2
+            // are made, and for those both query tiles were done with tile j - 3 and its note.)
+            const int key = kbegin + j * FA_BN + lane * ps;
+            const bool there = page >= 0 && source >= 0 && (p.listed == nullptr || source < p.listed_pages);
+            const unsigned gone = __ballot_sync(0xffffffffu, lane < pages_per_tile && key < kend && key + ps > first_seen && !there);
+            const unsigned groups = __ballot_sync(0xffffffffu, lane < FA_BN / 8 && ((gone >> (8 * lane / ps)) & 1u));
+            if (lane == 0) {
+                missing_keys[j % FA_NOTES] = groups;
+                fa_mbar_arrive(&noted[j % FA_NOTES]);
+            }
             page = next_page;
         }
     } else if (warp == 1) {
@@ -501,12 +529,15 @@ attn_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             bool alive = true;
             for (int j = 0; j < num_tiles && alive; ++j) {
                 const int k0 = kbegin + j * FA_BN;
+                if (!fa_mbar_wait(&noted[j % FA_NOTES], (j / FA_NOTES) & 1, (6u << 24) | (x << 20) | j, failed)) { alive = false; break; }
+                const unsigned missing = missing_keys[j % FA_NOTES];
                 if (!fa_mbar_wait(&s_full[x], j & 1, (5u << 24) | (x << 20) | j, failed)) { alive = false; break; }
                 fa_fence_after();
                 const bool full_tile = k0 + FA_BN - 1 <= xpos_first && k0 >= xlo_last && k0 + FA_BN <= kend;
                 float v[FA_BN];
                 fa_row_load(tmem_s, v);
                 if (!full_tile) fa_row_mask(v, k0, pos_r, lo_r, kend);
+                if (missing != 0u) fa_row_drop(v, missing);
                 const float mx = fa_row_max(v) * p.scale_log2;         // the scale is positive
                 // The reference point of the exponentials moves only when the maximum grew by more than 2^8:
                 // probabilities stay below 256, and the running output is rescaled rarely.
@@ -1449,6 +1480,7 @@ struct FaArgs {
     const int* block_table; long long bt_stride; const int* seg_off; const int* seg_slot; const int* seg_start; const int* seg_len;
     void* out; long long num_segments, max_seg_len, nq, nkv, page_size, window, splits;
     float* part_acc; float* part_ml; const int* token_seg; long long num_tokens;
+    const int* listed; long long listed_pages;
     double scale;
 };
 
@@ -1481,6 +1513,7 @@ PI_EXPORT int pi_attention_tcgen05(const FaArgs* args, cudaStream_t stream) {
     if (rc) return rc;
     FaParams p;
     p.q = (const bf16*)q; p.q_stride = q_stride; p.block_table = a.block_table; p.bt_stride = bt_stride;
+    p.listed = a.listed; p.listed_pages = a.listed_pages; p.copies = a.num_pages;
     p.seg_off = a.seg_off; p.seg_slot = a.seg_slot; p.seg_start = a.seg_start; p.seg_len = a.seg_len;
     p.out = (bf16*)out; p.nq = nq; p.nkv = nkv; p.group = nq / nkv; p.page_size = page_size; p.window = window;
     p.scale_log2 = scale * 1.4426950408889634f;
@@ -1493,7 +1526,7 @@ PI_EXPORT int pi_attention_tcgen05(const FaArgs* args, cudaStream_t stream) {
     int device = 0;
     if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return pi_refuse("pi_attention_tcgen05: no current device below 64");
     constexpr unsigned tile_bytes = (PI_HEAD_DIM / 64) * 128 * 128;
-    const size_t smem = (size_t)(2 + FA_STAGES) * tile_bytes + (2 * FA_STAGES + 6) * 8 + 16 + 1024;
+    const size_t smem = (size_t)(2 + FA_STAGES) * tile_bytes + (2 * FA_STAGES + 6 + FA_NOTES) * 8 + (2 + FA_NOTES) * 4 + 1024;
     auto kernel = attn_tcgen05_kernel<PI_HEAD_DIM>;
     if (!configured[device]) {
         cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);

@@ -241,7 +241,8 @@ def attention_decode_8bit(q: torch.Tensor, q_stride: int, kcache: torch.Tensor, 
                           out: torch.Tensor | None = None, span_min: int | None = None,
                           pair_cost: int | None = None) -> torch.Tensor:
     """Single tokens over 8-bit pages (csrc/attention_8bit.cu): segments of one token, whose keys and values - the newest
-    included - are in the pages.  ``q`` holds the normalised, rotated query heads of token t at element offset t * q_stride.
+    included - are in the pages; keys of pages that are not there are left out of the softmax, and a row that sees no key becomes
+    zeros.  ``q`` holds the normalised, rotated query heads of token t at element offset t * q_stride.
     Rows of segments of several tokens in ``out`` [num_tokens, nq d] are left as they are (``attention_prompt_8bit``).
     At most DECODE_8BIT_MAX_SEGMENTS segments; slices of the four seg_* tensors do for more.
     ``workspace`` (made here when missing): what CTAs leave for one another; launches that share one must not overlap."""
@@ -276,7 +277,8 @@ def attention_prompt_8bit(q: torch.Tensor, q_stride: int, kcache: torch.Tensor, 
     call may meet shorter ones, not longer ones).  ``keys`` /
     ``values``: bfloat16 [listed pages, kv heads, page size, d] for the copies, made here when missing; the layers of a step
     can share them.  Rows of single-token segments in ``out`` [num_tokens, nq d] are left as they are, and segments' tokens
-    behind the first ``num_tokens`` are left out."""
+    behind the first ``num_tokens`` are left out.  Keys of pages that the block table or the pool does not have are left out
+    of the softmax, as ``attention_decode_8bit`` leaves them out; a row that sees no key at all becomes zeros."""
     device = _on_current_device((q, kcache, vcache, kscale, vscale, seg_start, seg_len, out, keys, values, maps.page_list, maps.table))
     code, pages, _, page_size, d = _check_pools(kcache, vcache, kscale, vscale, head_dim, nkv)
     if maps.table is None:
@@ -323,5 +325,5 @@ def attention_prompt_8bit(q: torch.Tensor, q_stride: int, kcache: torch.Tensor, 
     _k._PROMPT(device, (q.data_ptr(), q_stride, where[0], where[1], N, maps.table.data_ptr(), W, maps.seg_off.data_ptr(),
                         maps.rows.data_ptr(), seg_start.data_ptr(), seg_len.data_ptr(), out.data_ptr(), R, longest, nq, nkv, page_size,
                         window or 0, splits, at if rows else 0, at + rows * 4 * d if rows else 0, maps.token_seg.data_ptr(), num_tokens,
-                        scale), launches=2 if splits > 1 else 1, head_dim=d)
+                        maps.page_list.data_ptr(), pages, scale), launches=2 if splits > 1 else 1, head_dim=d)
     return out

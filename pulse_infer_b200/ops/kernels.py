@@ -114,7 +114,7 @@ class _Record:
         _check(lib, fn(self.pack(*args), *extra, stream), self.name, launches)
 
 
-_PROMPT = _Record("attention_tcgen05", "pi_attention_tcgen05", 23, 1)
+_PROMPT = _Record("attention_tcgen05", "pi_attention_tcgen05", 25, 1)
 
 
 def _need_cuda(*tensors) -> None:
@@ -414,7 +414,7 @@ def attention_tcgen05(q: torch.Tensor, q_stride: int, kcache, vcache, block_tabl
                             block_table.shape[1], seg_off.data_ptr(), seg_slot.data_ptr(), seg_start.data_ptr(), seg_len.data_ptr(),
                             out.data_ptr(), num_segments, max_seg_len, nq, nkv, page_size, window or 0, splits,
                             part_acc.data_ptr() if splits > 1 else 0, part_ml.data_ptr() if splits > 1 else 0,
-                            token_seg.data_ptr() if splits > 1 else 0, num_tokens, scale),
+                            token_seg.data_ptr() if splits > 1 else 0, num_tokens, 0, 0, scale),
             launches=2 if splits > 1 else 1, head_dim=head_dim)
     return out
 

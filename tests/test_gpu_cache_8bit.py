@@ -728,3 +728,45 @@ def test_calls_without_tokens():
         ops.attention_decode_8bit(q, 256, *pools, torch.zeros(2, 2, dtype=torch.int32, device=dev), i32(0, 0), i32(0, 1), i32(*start),
                                   i32(*length), 3, 2, 4, 2, 64, None, 0.1, out=out)
         assert (out == 5).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nq,nkv,d,page,window", [(8, 2, 128, 16, None), (4, 4, 64, 64, None), (6, 2, 64, 16, 90), (4, 1, 128, 128, None)])
+def test_portions_over_missing_pages(dtype, nq, nkv, d, page, window):
+    """Pages that are not in the block table, or not in the pool, are left out of the softmax, as single tokens leave them out: in
+    the middle of a context, at its beginning, under the portion itself; with shares of the keys and without; all of them."""
+    dev, ops = need_gpu(), _ops()
+    for portions in ([(300, 40), (0, 200), (257, 3), (64, 70)], [(3000, 20), (700, 5)]):
+        lengths = [a + n for a, n in portions]
+        seqs = Sequences(lengths, nkv, d, page, dtype, seed=page + nq)
+        table = seqs.table.clone()
+        rng = np.random.RandomState(d + page)
+        for s in range(len(lengths)):
+            used = (lengths[s] + page - 1) // page
+            for i in range(used):
+                if rng.rand() < 0.3:
+                    table[s, i] = [-1, 10 ** 6, seqs.pools.pages][rng.randint(3)]
+        table[1, :] = -1                                   # nothing of it is there
+        table[0, 0] = -1                                   # neither are the first keys of this one
+        i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+        T = sum(n for _, n in portions)
+        start, length = i32([a for a, _ in portions]), i32([n for _, n in portions])
+        listed = sum((a + n - 1) // page - (max(0, a - window + 1) // page if window else 0) + 1 for a, n in portions)
+        maps = ops.page_maps(table.to(dev), i32(list(range(len(portions)))), start, length, page, T, num_listed_pages=listed, window=window, min_tokens=2)
+        q = torch.randn(T, nq * d, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+        pools = seqs.pools.on(dev)
+        out = ops.attention_prompt_8bit(q.to(dev), nq * d, *pools, maps, start, length, portions, T, nq, nkv, d, window, d ** -0.5)
+        assert ops.attention_tcgen05_loaded_status() == 0
+        got, t = out.cpu().double().view(T, nq, d), 0
+        for s, (a, n) in enumerate(portions):
+            there = [0 <= int(table[s, i // page]) < seqs.pools.pages for i in range(a + n)]
+            for i in sorted({0, 1, n // 2, n - 2, n - 1} | set(range(0, n, 17))):
+                lo = max(0, a + i - window + 1) if window else 0
+                keep = [x for x in range(lo, a + i + 1) if there[x]]
+                if not keep:
+                    assert (got[t + i] == 0).all(), (s, i)
+                    continue
+                want, bound = attention_with_bound(q[t + i].double().view(nq, d), seqs.k[s][keep], seqs.v[s][keep], seqs.vs[s][keep], len(keep) - 1,
+                                                   None, d ** -0.5, BF16_HALF_STEP, d, BF16_HALF_STEP)
+                assert ((got[t + i] - want).abs() <= bound).all(), (s, i, ((got[t + i] - want).abs() / bound).max())
+            t += n
