@@ -288,7 +288,7 @@ def attention_prompt_8bit(q: torch.Tensor, q_stride: int, kcache: torch.Tensor, 
     _vector("seg_start", seg_start, torch.int32, (R,))
     _vector("seg_len", seg_len, torch.int32, (R,))
     portions = [p for p in portions if p[1] > 1]
-    if not portions:
+    if not portions or num_tokens == 0:
         return out
     longest = need = 0
     for start, n in portions:

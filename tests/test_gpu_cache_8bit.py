@@ -770,3 +770,17 @@ def test_portions_over_missing_pages(dtype, nq, nkv, d, page, window):
                                                    None, d ** -0.5, BF16_HALF_STEP, d, BF16_HALF_STEP)
                 assert ((got[t + i] - want).abs() <= bound).all(), (s, i, ((got[t + i] - want).abs() / bound).max())
             t += n
+
+
+def test_prompt_attention_without_rows():
+    """Maps and queries of no tokens at all, with portions that would be cut into shares and without: nothing to do."""
+    dev, ops = need_gpu(), _ops()
+    nq, nkv, d, page = 8, 2, 64, 16
+    pools = ops.cache_8bit_pools(400, nkv, page, d, torch.int8, dev)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    for start in (0, 5000):
+        table = torch.arange(400, dtype=torch.int32, device=dev).view(1, 400)
+        maps = ops.page_maps(table, i32(0), i32(start), i32(30), page, 0, num_listed_pages=(start + 29) // page + 1, min_tokens=2)
+        q = torch.zeros(0, nq * d, dtype=torch.bfloat16, device=dev)
+        out = ops.attention_prompt_8bit(q, nq * d, *pools, maps, i32(start), i32(30), [(start, 30)], 0, nq, nkv, d, None, 0.1)
+        assert out.shape == (0, nq * d)
