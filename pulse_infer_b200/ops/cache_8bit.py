@@ -35,6 +35,11 @@ def _vector(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple | None 
                           f"{t.dtype} {tuple(t.shape)}")
 
 
+def _window(window: int | None) -> int:
+    """0: none.  Positions are 32-bit numbers, so a longer window is one that reaches everything."""
+    return min(window or 0, 2 ** 31 - 1)
+
+
 def cache_8bit_usable(head_dim: int, page_size: int) -> bool:
     return head_dim in (64, 128) and page_size in PAGE_SIZES_8BIT
 
@@ -125,7 +130,7 @@ def page_maps(block_table: torch.Tensor, seg_slot: torch.Tensor, seg_start: torc
         ptr.append(at)
         at += 4 * n
     _PAGE_MAPS(device, (block_table.data_ptr(), slots, W, seg_slot.data_ptr(), seg_start.data_ptr(), seg_len.data_ptr(), R, page_size,
-                        T, N, window or 0, min_tokens, ptr[0], ptr[1], ptr[2], ptr[4], ptr[5], ptr[6], ptr[3],
+                        T, N, _window(window), min_tokens, ptr[0], ptr[1], ptr[2], ptr[4], ptr[5], ptr[6], ptr[3],
                         ptr[7] if with_table else 0, ptr[8]))
     slot_map, positions, token_seg, page_tokens, seg_off, page_off, page_list, table, rows = flat.split_with_sizes(sizes)
     return PageMaps(slot_map.view(torch.int64), positions, token_seg, seg_off, page_off, page_list, page_tokens.view(N, 2),
@@ -262,7 +267,7 @@ def attention_decode_8bit(q: torch.Tensor, q_stride: int, kcache: torch.Tensor, 
                      seg_len.data_ptr(), out.data_ptr(), ws.acc.data_ptr(), ws.ml.data_ptr(), ws.count.data_ptr(), ws.ctas,
                      DECODE_8BIT_SPAN_MIN if span_min is None else span_min,
                      DECODE_8BIT_PAIR_COST if pair_cost is None else pair_cost, num_tokens, num_segments, nq, nkv, d, page_size,
-                     window or 0, scale))
+                     _window(window), scale))
     return out
 
 
@@ -324,6 +329,6 @@ def attention_prompt_8bit(q: torch.Tensor, q_stride: int, kcache: torch.Tensor, 
                    maps.page_list.data_ptr(), maps.page_tokens.data_ptr(), N, where[0], where[1]), launches=1 if N else 0)
     _k._PROMPT(device, (q.data_ptr(), q_stride, where[0], where[1], N, maps.table.data_ptr(), W, maps.seg_off.data_ptr(),
                         maps.rows.data_ptr(), seg_start.data_ptr(), seg_len.data_ptr(), out.data_ptr(), R, longest, nq, nkv, page_size,
-                        window or 0, splits, at if rows else 0, at + rows * 4 * d if rows else 0, maps.token_seg.data_ptr(), num_tokens,
+                        _window(window), splits, at if rows else 0, at + rows * 4 * d if rows else 0, maps.token_seg.data_ptr(), num_tokens,
                         maps.page_list.data_ptr(), pages, scale), launches=2 if splits > 1 else 1, head_dim=d)
     return out

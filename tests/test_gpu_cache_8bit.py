@@ -784,3 +784,23 @@ def test_prompt_attention_without_rows():
         q = torch.zeros(0, nq * d, dtype=torch.bfloat16, device=dev)
         out = ops.attention_prompt_8bit(q, nq * d, *pools, maps, i32(start), i32(30), [(start, 30)], 0, nq, nkv, d, None, 0.1)
         assert out.shape == (0, nq * d)
+
+
+def test_windows_beyond_32_bits():
+    """A window that no context reaches is no window, however large the number."""
+    dev, ops = need_gpu(), _ops()
+    nq, nkv, d, page = 4, 2, 64, 16
+    seqs = Sequences([200, 60], nkv, d, page, torch.int8)
+    pools, table = seqs.pools.on(dev), seqs.table.to(dev)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    q = torch.randn(11, nq * d, device=dev).to(torch.bfloat16)
+    results = []
+    for window in (None, 2 ** 31 - 1, 2 ** 31, 2 ** 32 + 5, 2 ** 63 - 1, 2 ** 70):
+        start, length = i32(190, 59), i32(10, 1)
+        maps = ops.page_maps(table, i32(0, 1), start, length, page, 11, num_listed_pages=13, window=window, min_tokens=2)
+        out = torch.zeros(11, nq * d, dtype=torch.bfloat16, device=dev)
+        ops.attention_prompt_8bit(q, nq * d, *pools, maps, start, length, [(190, 10)], 11, nq, nkv, d, window, 0.1, out=out)
+        ops.attention_decode_8bit(q, nq * d, *pools, table, maps.seg_off, i32(0, 1), start, length, 11, 2, nq, nkv, d, window, 0.1, out=out)
+        results.append((maps.page_list.clone(), maps.page_tokens.clone(), maps.table.clone(), out))
+    for other in results[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(results[0], other))
