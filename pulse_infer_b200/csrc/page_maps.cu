@@ -62,8 +62,9 @@ __global__ void __launch_bounds__(PM_THREADS) page_maps_kernel(const PmParams p)
     int* tok = pm_smem;
     int* pg = pm_smem + p.num_segments + 1;
     const int R = p.num_segments, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    // The kernel behind this one is not let in early: the attention kernels look at a step's offsets, slots and lengths before they
+    // wait for the kernel in front of them, which is right for what was there before the step, and this kernel writes some of it.
     pdl_wait();
-    pdl_trigger();
     int base_tok = 0, base_pg = 0;
     for (int first = 0; first < R; first += PM_THREADS) {
         const int r = first + threadIdx.x;

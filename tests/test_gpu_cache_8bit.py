@@ -804,3 +804,37 @@ def test_windows_beyond_32_bits():
         results.append((maps.page_list.clone(), maps.page_tokens.clone(), maps.table.clone(), out))
     for other in results[1:]:
         assert all(torch.equal(a, b) for a, b in zip(results[0], other))
+
+
+def test_page_maps_and_the_kernel_right_behind_them():
+    """The bf16 attention kernels read offsets and slots before they wait for the kernel in front of them; here that kernel is the
+    one that makes them, in memory that held the offsets of another step.  200 steps of two kinds in turn, no pause between."""
+    from gpu_util import PagedKV
+    dev, ops = need_gpu(), _ops()
+    nq, nkv, d, page = 8, 2, 128, 16
+    kinds = [[(0, 40, 30), (1, 0, 64), (2, 100, 20), (3, 7, 9)], [(3, 10, 6), (2, 60, 60), (0, 0, 41), (1, 64, 16)]]     # (slot, start, length)
+    kv = PagedKV([70, 80, 120, 16], nkv, d, page, torch.bfloat16, dev)
+    q = torch.randn(123, nq * d, device=dev).to(torch.bfloat16)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    metas = [[i32([s[k] for s in segs]) for k in range(3)] for segs in kinds]
+    # filler segments: their sums take the kernel a while
+    many = 2000
+    wide = [[torch.cat([x, torch.zeros(many, dtype=torch.int32, device=dev)]) for x in meta] for meta in metas]
+
+    def step(kind, out, pause):
+        slot, start, length = wide[kind]
+        maps = ops.page_maps(kv.table_dev, slot, start, length, page, 123, min_tokens=2, with_table=False)
+        if pause:
+            torch.cuda.synchronize()
+        ops.attention_tcgen05(q, nq * d, kv.kcache, kv.vcache, kv.table_dev, maps.seg_off, slot, start, length, 123, 4, 64, nq, nkv, d, page, None,
+                              d ** -0.5, out)
+
+    want, outs = ([torch.zeros(123, nq * d, dtype=torch.bfloat16, device=dev) for _ in range(n)] for n in (2, 200))
+    for kind in (0, 1):
+        step(kind, want[kind], True)
+    torch.cuda.synchronize()
+    for i in range(200):
+        step(i % 2, outs[i], False)
+    torch.cuda.synchronize()
+    assert ops.attention_tcgen05_loaded_status() == 0 and (want[0] != 0).any() and not torch.equal(*want)
+    assert all(torch.equal(out, want[i % 2]) for i, out in enumerate(outs))
