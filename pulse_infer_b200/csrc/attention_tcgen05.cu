@@ -305,17 +305,22 @@ attn_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     constexpr unsigned S_COL = 0, O_COL = 256;           // S of query tile x at S_COL + 128 x (P over its first 64 columns), O at O_COL + 128 x
 
     // ---- which rows -------------------------------------------------------------------------------------
+    // (Read before pdl_wait(): the step's offsets, lengths, starts and slots are from before the step, or from a kernel that does
+    // not let the next one in early, as page_maps.  The first CTA waits even if it has nothing to do: if that holds for all of
+    // them, in a replayed step of single tokens, the kernel would end, and let the next one go on, before the one in front of it.)
     const int kvh = blockIdx.x % p.nkv;
     const int rest = blockIdx.x / p.nkv;
     const int tile = p.tiles_per_seg - 1 - rest / p.num_segments;     // tiles with the most keys first
     const int seg = rest % p.num_segments;
     const int whole_len = p.seg_len[seg], tok_off = p.seg_off[seg];
-    if (whole_len == 1) return;                           // single tokens go to the decode kernel
-    const int len = min(whole_len, p.num_tokens - tok_off);          // tokens behind the last row of q and out are left out
-    const int G = p.group;
+    const int len = whole_len == 1 ? 0 : min(whole_len, p.num_tokens - tok_off);     // single tokens go to the decode kernel; tokens
+    const int G = p.group;                                                           // behind the last row of q and out are left out
     const int rows_total = len * G;
     const int row0 = tile * FA_ROWS;
-    if (row0 >= rows_total) return;
+    if (row0 >= rows_total) {
+        if (blockIdx.x == 0 && blockIdx.y == 0) pdl_wait();
+        return;
+    }
     const bool two = row0 + FA_BM < rows_total;           // the second query tile has rows
     const int start = p.seg_start[seg];
     const int* table = p.block_table + (size_t)p.seg_slot[seg] * p.bt_stride;
@@ -378,7 +383,7 @@ attn_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     __syncthreads();
     fa_fence_after();
     const unsigned tmem_base = *tmem_slot;
-    pdl_wait();   // q and the pages are written by the kernels before this one; all above touched this CTA only
+    pdl_wait();   // q and the pages are written by the kernels before this one; all above touched this CTA and the step's metadata only
     // Q: each of the eight softmax warps copies 32 rows, whole rows at a time, into the swizzled K-major layout (16-byte chunk
     // c of a 128-byte row goes to chunk c ^ (row & 7)); a row per thread took 4.4 to 6 us instead of 1.3 to 2.3
     if (warp >= 2) {

@@ -45,8 +45,9 @@ PI_EXPORT const char* pi_last_error() { return g_pi_error; }
 // Kernels are launched with "programmatic stream serialization": a kernel may be scheduled while the tail of
 // the kernel before it (in the same stream) is still running, and waits at pdl_wait() until that kernel has
 // completed and its writes are visible.  Everything a kernel does before pdl_wait() must therefore touch only
-// memory that no earlier kernel of the step writes (weights); every kernel calls pdl_wait() before its first
-// read of an activation and before its first write.  pdl_trigger() tells the runtime that the next kernel may
+// memory that no earlier kernel of the step writes (weights), or writes in a kernel that has ended by then (the
+// step's metadata: page_maps does not call pdl_trigger()); every kernel calls pdl_wait() before its first
+// read of an activation and before its first write, and in one CTA at least.  pdl_trigger() tells the runtime that the next kernel may
 // be scheduled as soon as all CTAs of this one have started.  After a copy or a library kernel the attribute
 // has no effect, and without it both calls do nothing.  PULSE_PDL=0 in the environment turns it off.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }

@@ -838,3 +838,49 @@ def test_page_maps_and_the_kernel_right_behind_them():
     torch.cuda.synchronize()
     assert ops.attention_tcgen05_loaded_status() == 0 and (want[0] != 0).any() and not torch.equal(*want)
     assert all(torch.equal(out, want[i % 2]) for i, out in enumerate(outs))
+
+
+def test_a_recorded_step_replayed_with_single_tokens_only():
+    """The prompt kernel then finds nothing to do in any CTA; pages, queries and single tokens around it come out as launched."""
+    dev, ops = need_gpu(), _ops()
+    nq, nkv, d, page, T = 8, 2, 128, 16, 50
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    table = torch.randperm(2 * 200, generator=torch.Generator().manual_seed(6)).int().view(2, 200).to(dev)
+    old = Pools(2 * 200, nkv, page, d, torch.int8, seed=5).on(dev)
+    old[2].fill_(2.0 ** -5); old[3].fill_(2.0 ** -6)
+    pools = [x.clone() for x in old]
+    slot, start, length = i32([0, 1]), i32([3000, 77]), i32([40, 10])
+    qkv = torch.randn(T, (nq + 2 * nkv) * d, device=dev).to(torch.bfloat16)
+    err = torch.zeros(1, dtype=torch.int32, device=dev)
+    ws = ops.attention_decode_workspace(d, dev)
+    out = torch.zeros(T, nq * d, dtype=torch.bfloat16, device=dev)
+
+    def step():
+        out.fill_(4.0)
+        maps = ops.page_maps(table, slot, start, length, page, T, num_listed_pages=200, min_tokens=2)
+        q = ops.qk_norm_rope_write_8bit(qkv, None, None, 1e-6, None, None, True, *pools, maps.slot_map, nq, nkv, d, err)
+        ops.attention_prompt_8bit(q, nq * d, *pools, maps, start, length, [(3000, 40), (77, 10)], T, nq, nkv, d, None, d ** -0.5, out=out)
+        ops.attention_decode_8bit(q, nq * d, *pools, table, maps.seg_off, slot, start, length, T, 2, nq, nkv, d, None, d ** -0.5,
+                                  workspace=ws, out=out)
+
+    def back():
+        for x, y in zip(pools, old):
+            x.view(torch.uint8).copy_(y.view(torch.uint8))
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for lengths in ([1, 1], [40, 10], [1, 1], [0, 1], [1, 0], [0, 0]):
+        length.copy_(i32(lengths))
+        results = []
+        for run in (step, graph.replay, graph.replay):
+            back()
+            run()
+            torch.cuda.synchronize()
+            results.append([out.clone()] + [x.view(torch.uint8).clone() for x in pools])
+        assert (results[0][0][sum(lengths):] == 4).all() and not (results[0][0][:sum(lengths)] == 4).all(1).any()
+        for again in results[1:]:
+            assert all(torch.equal(x, y) for x, y in zip(results[0], again))
+    assert ops.attention_tcgen05_loaded_status() == 0
