@@ -314,3 +314,24 @@ def test_a_grammar_that_fails_ends_its_own_request_only(model_folders, lookahead
     assert engine.get_result(free) == alone and len(engine.get_result(good)) == 6
     assert [t % 7 for t in engine.get_result(good)[:4]] == [0, 1, 2, 3]
     assert engine.generate([[4, 5]], 7, ignore_eos=True)[0] == alone and list(engine.get_stats().free_pages) == [60]
+
+
+def test_engine_applies_repetition_penalties_to_prompt_and_output(model_folders):
+    """Greedy tokens of an engine against a loop on the host that penalises the logits which the engine saw."""
+    from pulse_infer_b200 import Engine
+    need_gpu()
+    engine = Engine(model_folders["A"], dtype="float32", page_size=8, num_pages=40, max_batch_size=4)
+    plain = engine.generate([[4, 5, 6]], 16, ignore_eos=True)[0]
+    for kw in (dict(repetition_penalty=1.5), dict(repetition_penalty=1e6), dict(repetition_penalty=0.5), dict(repetition_penalty=1.2, presence_penalty=0.3)):
+        seen = []
+        engine.engine.logits_hook = lambda reqs, logits: seen.append(logits[0].double().cpu().numpy())
+        out = engine.generate([[4, 5, 6]], 16, ignore_eos=True, **kw)[0]
+        engine.engine.logits_hook = None
+        history = [4, 5, 6]
+        for x, token in zip(seen, out):
+            for t in set(history):
+                x[t] = (x[t] / kw["repetition_penalty"] if x[t] > 0 else x[t] * kw["repetition_penalty"]) - kw.get("presence_penalty", 0.0)
+            assert token == int(np.argmax(x))
+            history.append(token)
+        # a penalty of 1e6 leaves no token that was there; the mild ones need not change what this model repeats
+        assert len(seen) == len(out) == 16 and (kw["repetition_penalty"] < 1e6 or (out != plain and len(set(out)) == 16))
