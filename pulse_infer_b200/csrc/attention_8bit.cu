@@ -605,7 +605,8 @@ PI_EXPORT int pi_attention_decode_8bit(const A8Args* args, cudaStream_t stream) 
     if (cache_dtype != PI_E4M3 && cache_dtype != PI_INT8) return pi_refuse("pi_attention_decode_8bit: unknown dtype code %d of the pages", cache_dtype);
     if (window < 0 || bt_rows <= 0 || bt_stride <= 0) return pi_refuse("pi_attention_decode_8bit: window=%d, block table [%d, %d]", window, bt_rows, bt_stride);
     if (ws_ctas <= 0 || ws_ctas > 256 || a.ws_acc == nullptr || a.ws_ml == nullptr || a.ws_count == nullptr) return pi_refuse("pi_attention_decode_8bit: the workspace is missing (or for more than 256 CTAs: %d)", ws_ctas);
-    if (span_min < 1 || pair_cost < 0 || pair_cost > 64) return pi_refuse("pi_attention_decode_8bit: span_min=%d must be at least 1 and pair_cost=%d between 0 and 64", span_min, pair_cost);
+    // (span_min and the units, at most 10^9 each, are added up in 32 bits)
+    if (a.span_min < 1 || a.span_min > 1000000000LL || a.pair_cost < 0 || a.pair_cost > 64) return pi_refuse("pi_attention_decode_8bit: span_min=%lld must lie between 1 and 10^9 and pair_cost=%lld between 0 and 64", a.span_min, a.pair_cost);
     if (q_stride % 8 != 0 || (((uintptr_t)a.q | (uintptr_t)a.kcache | (uintptr_t)a.vcache) & 15) || ((uintptr_t)a.out & 7))
         return pi_refuse("pi_attention_decode_8bit: q and the pages must start on 16-byte boundaries, the output on an 8-byte one, and q needs a stride that is a multiple of 8");
     const long long blocks = a.num_pages * nkv * (page_size / C8_BLOCK);

@@ -130,7 +130,7 @@ def page_maps(block_table: torch.Tensor, seg_slot: torch.Tensor, seg_start: torc
         ptr.append(at)
         at += 4 * n
     _PAGE_MAPS(device, (block_table.data_ptr(), slots, W, seg_slot.data_ptr(), seg_start.data_ptr(), seg_len.data_ptr(), R, page_size,
-                        T, N, _window(window), min_tokens, ptr[0], ptr[1], ptr[2], ptr[4], ptr[5], ptr[6], ptr[3],
+                        T, N, _window(window), min(min_tokens, 2 ** 31 - 1), ptr[0], ptr[1], ptr[2], ptr[4], ptr[5], ptr[6], ptr[3],
                         ptr[7] if with_table else 0, ptr[8]))
     slot_map, positions, token_seg, page_tokens, seg_off, page_off, page_list, table, rows = flat.split_with_sizes(sizes)
     return PageMaps(slot_map.view(torch.int64), positions, token_seg, seg_off, page_off, page_list, page_tokens.view(N, 2),

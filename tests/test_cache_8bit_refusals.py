@@ -38,3 +38,28 @@ def test_histories_beyond_the_counter_are_refused():
         record = kernels._LOGIT_RULES.pack(0, 8, 0, 8, 1, 8, 0, 0, history, 0, 0, 0, 0, 0, 0, 0, biases, 0, 0, 0)
         assert launch(record, None) == -1, (history, biases)
         assert b"beyond the limit" in lib.pi_last_error()
+
+
+def test_shares_that_32_bits_do_not_hold_are_refused():
+    """The number of CTAs is (units + span_min - 1) / span_min: with a span near 2^31 the sum wrapped, and no CTA did anything.
+    (Refused before the launcher looks at the device.)"""
+    from pulse_infer_b200.ops import cache_8bit, kernels
+    lib = kernels._lib("attention_8bit")
+    launch = lib.pi_attention_decode_8bit
+    launch.argtypes = cache_8bit._DECODE.argtypes
+    for span_min, pair_cost in ((2 ** 31 - 1, 2), (1000000001, 2), (2 ** 32 + 2, 2), (-2 ** 32 + 2, 2), (2, 2 ** 32), (0, 2), (2, -1)):
+        record = cache_8bit._DECODE.pack(16, 64, 16, 16, 16, 16, cache_8bit.INT8, 1, 16, 1, 1, 16, 16, 16, 16, 16, 16, 16, 16, 148, span_min, pair_cost,
+                                         1, 1, 1, 1, 64, 16, 0, 0.1)
+        assert launch(record, None) == -1
+        assert b"span_min" in lib.pi_last_error(), (span_min, pair_cost, lib.pi_last_error())
+
+
+def test_page_maps_hand_large_limits_on_as_what_they_mean(monkeypatch):
+    from pulse_infer_b200.ops import cache_8bit
+    seen = []
+    monkeypatch.setattr(cache_8bit, "_on_current_device", lambda tensors: 0)
+    monkeypatch.setattr(cache_8bit, "_PAGE_MAPS", lambda device, args: seen.append(args))
+    i32 = lambda *shape: torch.zeros(shape, dtype=torch.int32)  # noqa: E731
+    for window, min_tokens in ((2 ** 32 + 5, 2 ** 32 + 1), (2 ** 31, 2 ** 31), (7, 2)):
+        cache_8bit.page_maps(i32(2, 3), i32(2), i32(2), i32(2), 16, 2, window=window, min_tokens=min_tokens)
+    assert [a[10:12] for a in seen] == [(2 ** 31 - 1, 2 ** 31 - 1)] * 2 + [(7, 2)]
