@@ -48,7 +48,6 @@
 #define FA_ROWS 256          // rows of a CTA: two query tiles
 #define FA_BN 128            // keys of a tile
 #define FA_STAGES 5          // ring of K / V tiles
-#define FA_NOTES 4           // ring of notes of missing keys; three are in use at a time
 #define FA_THREADS 320
 #define FA_SPIN_LIMIT (1u << 22)
 
@@ -57,8 +56,8 @@ __device__ unsigned g_fa_status;
 struct FaParams {
     const bf16* q; int q_stride;
     const int* block_table; int bt_stride;
-    // pages that are copies: place i < copies holds a copy of page listed[i] of a pool of listed_pages, and is missing if that
-    // is not there.  Null: the pages are the pool's.
+    // pages that are copies: place i < copies holds a copy of page listed[i] of a pool of listed_pages; if that is not there, or
+    // no copy is named, the keys are missing.  Null: the pages are the pool's, and all that can be seen are there
     const int* listed; long long listed_pages; long long copies;
     const int* seg_off; const int* seg_slot; const int* seg_start; const int* seg_len;
     bf16* out;
@@ -295,7 +294,9 @@ struct FaRow {
     }
 };
 
-template <int D>
+// COPIES: the pages are copies, some of which may be missing (FaParams).  A kernel of its own: the look-up takes 1.6 us of 50 for
+// 2,039 tokens, and plain pages need none of it.
+template <int D, bool COPIES>
 __global__ void __launch_bounds__(FA_THREADS, 1)
 attn_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const FaParams p) {
     constexpr int HALVES = D / 64;                       // 64-wide (128-byte) column blocks of the head
@@ -306,21 +307,25 @@ attn_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 
     // ---- which rows -------------------------------------------------------------------------------------
     // (Read before pdl_wait(): the step's offsets, lengths, starts and slots are from before the step, or from a kernel that does
-    // not let the next one in early, as page_maps.  The first CTA waits even if it has nothing to do: if that holds for all of
-    // them, in a replayed step of single tokens, the kernel would end, and let the next one go on, before the one in front of it.)
+    // not let the next one in early, as page_maps.  With copied pages the first CTA waits even if it has nothing to do: if that holds
+    // for all of them, in a replayed step of single tokens, the kernel would end, and let the next one go on, before the kernel
+    // that makes the copies.  It costs 2 us in a step with 31 single tokens; a step over plain pages is not recorded with portions.)
     const int kvh = blockIdx.x % p.nkv;
     const int rest = blockIdx.x / p.nkv;
     const int tile = p.tiles_per_seg - 1 - rest / p.num_segments;     // tiles with the most keys first
     const int seg = rest % p.num_segments;
     const int whole_len = p.seg_len[seg], tok_off = p.seg_off[seg];
-    const int len = whole_len == 1 ? 0 : min(whole_len, p.num_tokens - tok_off);     // single tokens go to the decode kernel; tokens
-    const int G = p.group;                                                           // behind the last row of q and out are left out
+    const bool first_cta = COPIES && (blockIdx.x | blockIdx.y) == 0;
+    if (whole_len == 1 && !first_cta) return;             // single tokens go to the decode kernel
+    const int len = min(whole_len, p.num_tokens - tok_off);          // tokens behind the last row of q and out are left out
+    const int G = p.group;
     const int rows_total = len * G;
     const int row0 = tile * FA_ROWS;
-    if (row0 >= rows_total) {
-        if (blockIdx.x == 0 && blockIdx.y == 0) pdl_wait();
+    if (first_cta && (whole_len == 1 || row0 >= rows_total)) {
+        pdl_wait();
         return;
     }
+    if (row0 >= rows_total) return;
     const bool two = row0 + FA_BM < rows_total;           // the second query tile has rows
     const int start = p.seg_start[seg];
     const int* table = p.block_table + (size_t)p.seg_slot[seg] * p.bt_stride;
@@ -359,14 +364,11 @@ attn_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     unsigned long long* s_full = bars + 2 * FA_STAGES;    // [2] MMA -> softmax of query tile x: scores are in TMEM
     unsigned long long* p_ready = s_full + 2;             // [2] softmax (4 warps) -> MMA: P written, O rescaled, S read
     unsigned long long* pv_done = s_full + 4;             // [2] MMA -> softmax: the last product with the values is done
-    unsigned long long* noted = s_full + 6;               // [FA_NOTES] TMA warp -> softmax: the tile's missing keys are noted
-    unsigned* tmem_slot = reinterpret_cast<unsigned*>(noted + FA_NOTES);
+    unsigned* tmem_slot = reinterpret_cast<unsigned*>(s_full + 6);
     volatile unsigned* failed = tmem_slot + 1;
-    volatile unsigned* missing_keys = tmem_slot + 2;      // [FA_NOTES] eight keys to a bit
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < FA_NOTES; ++i) fa_mbar_init(&noted[i], 1);
         for (int i = 0; i < FA_STAGES; ++i) { fa_mbar_init(&full[i], 1); fa_mbar_init(&empty[i], 1); }
         for (int i = 0; i < 2; ++i) { fa_mbar_init(&s_full[i], 1); fa_mbar_init(&p_ready[i], 4); fa_mbar_init(&pv_done[i], 1); }
         *failed = 0;
@@ -384,6 +386,20 @@ attn_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     fa_fence_after();
     const unsigned tmem_base = *tmem_slot;
     pdl_wait();   // q and the pages are written by the kernels before this one; all above touched this CTA and the step's metadata only
+    // With copied pages: is some page missing whose keys a query of this CTA should see?  Such keys are left out of the softmax,
+    // whatever the ring holds in their place.  The softmax warps look through all pages of the CTA once, while the queries are on
+    // their way, and page by page only if one is missing.  (A note for every tile from the TMA warp cost 4 to 7 % of all calls.)
+    const int first_seen = fa_window_lo(pos_first, p.window);
+    auto there = [&](int index) -> bool {
+        const int copy = index < p.bt_stride ? table[index] : -1;
+        const int source = copy >= 0 && copy < p.copies ? p.listed[copy] : -1;
+        return source >= 0 && source < p.listed_pages;
+    };
+    bool any_missing = false;
+    if (COPIES && warp >= 2) {
+        const int last = min(kend, kbegin + num_tiles * FA_BN) - 1;
+        for (int i = max(first_seen, kbegin) / p.page_size + threadIdx.x - 64; i <= last / p.page_size; i += FA_THREADS - 64) any_missing |= !there(i);
+    }
     // Q: each of the eight softmax warps copies 32 rows, whole rows at a time, into the swizzled K-major layout (16-byte chunk
     // c of a 128-byte row goes to chunk c ^ (row & 7)); a row per thread took 4.4 to 6 us instead of 1.3 to 2.3
     if (warp >= 2) {
@@ -411,7 +427,14 @@ attn_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     }
     if (warp > 0) {               // the producer does not wait for the queries
         fa_fence_async_smem();    // generic-proxy writes above become visible to tcgen05.mma
-        asm volatile("bar.sync 1, %0;" ::"n"(FA_THREADS - 32) : "memory");
+        if constexpr (!COPIES) {
+            asm volatile("bar.sync 1, %0;" ::"n"(FA_THREADS - 32) : "memory");
+        } else {
+            unsigned some;
+            asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 p, %1, 0;\nbarrier.cta.red.or.pred q, 1, %2, p;\nselp.u32 %0, 1, 0, q;\n}"
+                         : "=r"(some) : "r"((unsigned)any_missing), "n"(FA_THREADS - 32) : "memory");
+            any_missing = some != 0u;
+        }
     }
 
     if (warp == 0) {
@@ -424,12 +447,9 @@ attn_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             const int key = kbegin + j * FA_BN + lane * ps;
             return (j < num_tiles && lane < pages_per_tile && key < kend && key / ps < p.bt_stride) ? table[key / ps] : -1;
         };
-        const int first_seen = fa_window_lo(pos_first, p.window);
         int page = lookup(0);
         for (int j = 0; j < num_tiles && !*failed; ++j) {
             const int next_page = lookup(j + 1);
-            int source = 0;                                // needed below, when the loads are on their way
-            if (p.listed != nullptr) source = page >= 0 && page < p.copies ? p.listed[page] : -1;
             const unsigned mask = __ballot_sync(0xffffffffu, page >= 0);
             const unsigned bytes = (unsigned)__popc(mask) * page_bytes * HALVES;
             const int row = (page * p.nkv + kvh) * ps;
@@ -447,17 +467,6 @@ attn_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                 }
             }
             if (!ok) break;
-            // A page that some query of the block should see and that is not there: its keys are left out of the softmax, whatever
-            // the ring holds in their place.  (A slot of the notes is free again: V(j) was asked for, so the scores of tile j - 2
-            // are made, and for those both query tiles were done with tile j - 3 and its note.)
-            const int key = kbegin + j * FA_BN + lane * ps;
-            const bool there = page >= 0 && source >= 0 && (p.listed == nullptr || source < p.listed_pages);
-            const unsigned gone = __ballot_sync(0xffffffffu, lane < pages_per_tile && key < kend && key + ps > first_seen && !there);
-            const unsigned groups = __ballot_sync(0xffffffffu, lane < FA_BN / 8 && ((gone >> (8 * lane / ps)) & 1u));
-            if (lane == 0) {
-                missing_keys[j % FA_NOTES] = groups;
-                fa_mbar_arrive(&noted[j % FA_NOTES]);
-            }
             page = next_page;
         }
     } else if (warp == 1) {
@@ -534,15 +543,17 @@ attn_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             bool alive = true;
             for (int j = 0; j < num_tiles && alive; ++j) {
                 const int k0 = kbegin + j * FA_BN;
-                if (!fa_mbar_wait(&noted[j % FA_NOTES], (j / FA_NOTES) & 1, (6u << 24) | (x << 20) | j, failed)) { alive = false; break; }
-                const unsigned missing = missing_keys[j % FA_NOTES];
                 if (!fa_mbar_wait(&s_full[x], j & 1, (5u << 24) | (x << 20) | j, failed)) { alive = false; break; }
                 fa_fence_after();
                 const bool full_tile = k0 + FA_BN - 1 <= xpos_first && k0 >= xlo_last && k0 + FA_BN <= kend;
                 float v[FA_BN];
                 fa_row_load(tmem_s, v);
                 if (!full_tile) fa_row_mask(v, k0, pos_r, lo_r, kend);
-                if (missing != 0u) fa_row_drop(v, missing);
+                if (COPIES && any_missing) {
+                    const int key = k0 + lane * p.page_size;
+                    const unsigned gone = __ballot_sync(0xffffffffu, key < k0 + FA_BN && key < kend && key + p.page_size > first_seen && !there(key / p.page_size));
+                    if (gone != 0u) fa_row_drop(v, __ballot_sync(0xffffffffu, lane < FA_BN / 8 && ((gone >> (8 * lane / p.page_size)) & 1u)));
+                }
                 const float mx = fa_row_max(v) * p.scale_log2;         // the scale is positive
                 // The reference point of the exponentials moves only when the maximum grew by more than 2^8:
                 // probabilities stay below 256, and the running output is rescaled rarely.
@@ -1527,19 +1538,20 @@ PI_EXPORT int pi_attention_tcgen05(const FaArgs* args, cudaStream_t stream) {
     p.splits = splits; p.part_acc = part_acc; p.part_ml = part_ml;
     const long long ctas = (long long)num_segments * p.tiles_per_seg * nkv;
     if (ctas > 2147483647LL) return pi_refuse("pi_attention_tcgen05: %lld tiles are beyond the grid limit", ctas);
-    static bool configured[64] = {};                          // per device: the attribute belongs to a device's copy of the kernel
+    static bool configured[2][64] = {};                       // per device: the attribute belongs to a device's copy of the kernel
     int device = 0;
     if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return pi_refuse("pi_attention_tcgen05: no current device below 64");
     constexpr unsigned tile_bytes = (PI_HEAD_DIM / 64) * 128 * 128;
-    const size_t smem = (size_t)(2 + FA_STAGES) * tile_bytes + (2 * FA_STAGES + 6 + FA_NOTES) * 8 + (2 + FA_NOTES) * 4 + 1024;
-    auto kernel = attn_tcgen05_kernel<PI_HEAD_DIM>;
-    if (!configured[device]) {
+    const size_t smem = (size_t)(2 + FA_STAGES) * tile_bytes + (2 * FA_STAGES + 6) * 8 + 16 + 1024;
+    const bool copied = a.listed != nullptr;
+    auto kernel = copied ? attn_tcgen05_kernel<PI_HEAD_DIM, true> : attn_tcgen05_kernel<PI_HEAD_DIM, false>;
+    if (!configured[copied][device]) {
         cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (err != cudaSuccess) {
             snprintf(g_pi_error, sizeof(g_pi_error), "pi_attention_tcgen05: cannot reserve %zu bytes of shared memory: %s", smem, cudaGetErrorString(err));
             return (int)err;
         }
-        configured[device] = true;
+        configured[copied][device] = true;
     }
     pi_launch(kernel, dim3((unsigned)ctas, (unsigned)splits), dim3(FA_THREADS), smem, stream, mk, mv, p);
     rc = pi_check_launch("pi_attention_tcgen05");
