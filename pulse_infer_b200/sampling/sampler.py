@@ -84,6 +84,8 @@ class Sampler:
                      allowed: list | None) -> torch.Tensor:
         """``logits`` after the rules of every row, in a new tensor."""
         n, V = logits.shape
+        if n > 1 and logits.stride(0) < V:               # a row that several requests share
+            logits = logits.contiguous()
         told = history is not None
         tokens = [np.asarray(history[i], dtype=np.int32) if told and p.needs_history else np.empty(0, np.int32)
                   for i, p in enumerate(params)]

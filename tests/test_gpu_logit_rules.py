@@ -335,3 +335,13 @@ def test_engine_applies_repetition_penalties_to_prompt_and_output(model_folders)
             history.append(token)
         # a penalty of 1e6 leaves no token that was there; the mild ones need not change what this model repeats
         assert len(seen) == len(out) == 16 and (kw["repetition_penalty"] < 1e6 or (out != plain and len(set(out)) == 16))
+
+
+def test_a_sampler_takes_rules_for_rows_that_share_their_logits():
+    """One row of logits expanded to several requests, as before there was a kernel for all rules."""
+    from pulse_infer_b200.sampling import Sampler, SamplingParams
+    dev = need_gpu()
+    x = torch.randn(1, 900, generator=torch.Generator().manual_seed(2))
+    first, second, third = x[0].topk(3).indices.tolist()
+    params = [SamplingParams(banned_tokens=(first,)), SamplingParams(), SamplingParams(banned_tokens=(first, second))]
+    assert Sampler(dev).sample(x.to(dev).expand(3, 900), params, [0] * 3) == [second, first, third]
