@@ -256,7 +256,9 @@ __device__ __forceinline__ void fa_add2(float& a, float& b, float x, float y) {
 }
 
 // p = 2^(s * scale - base) as bf16, two to a 32-bit column, written over the row's own scores (all of which are in
-// registers); returns the row's sum.
+// registers); returns the row's sum.  bf16 because both operands of the product with the values have one type; it rounds a weight by
+// up to 2^-8 of it and does not lose small ones as half precision would (weights lie up to 2^8 above the reference point, and far
+// below it).  The sum is of the weights before they are rounded.
 __device__ __forceinline__ float fa_row_probs(float (&v)[FA_BN], unsigned tmem_row, float scale_log2, float base) {
     float s0 = 0.0f, s1 = 0.0f, s2 = 0.0f, s3 = 0.0f;
     const float nbase = -base;

@@ -18,11 +18,14 @@
 // A block of four warps takes one key or value head of a run: the scale needs the whole run, at most 16 rows of D elements.
 // Lanes of D / 8 form a group that takes 16-byte pieces of one or two rows, so everything a run needs (rows, rotation, what lies
 // in the block) is asked for at once: the kernel is a chain of two round trips, the slots and the rest.  (One warp for all 16
-// rows went through the rotation tables of eight rows one after the other: 25 us instead of 12.)  A block looks for the
+// rows went through the rotation tables of eight rows one after the other: 25 us where this form took 12, before keys kept their
+// rounding errors; it takes 15.5 now.)  A block looks for the
 // runs that begin among `window` tokens: 16 in a step of many tokens - one run, as a rule - and 1 in a decode step.  Query heads
 // are plain streaming work; in a step of many tokens they are a kernel of their own, in a small one part of the same launch.
-// Measured (B200, 32 + 8 + 8 heads of 128): 20.6 us for 2,045 tokens, both kernels, 46 MB (2.2 TB/s: too few loads in flight per
-// warp, as in the bf16 kernel, and the arithmetic of the keys); 3.1 us for 8 decoding requests.
+// Measured (B200, 32 + 8 + 8 heads of 128, pairs of neighbours): 19.4 (e4m3) to 20.6 us (int8) for 2,045 tokens, both kernels,
+// 46 MB (2.2 TB/s: too few loads in flight per warp, as in the bf16 kernel, and the arithmetic of the keys); 3.1 us for 8
+// decoding requests.  Pairs of halves: 23.8 to 24.4 and 4.0 us; a lane then holds eight cosines and sines for each of its rows, and
+// 17 words of it are spilled from the 80 registers that six blocks per SM leave.
 // ---------------------------------------------------------------------------------------------------
 #define CW_WARPS 4
 #define CW_Q_ROWS 4          // query rows in flight per lane group

@@ -1,7 +1,7 @@
 // Token selection on the device from 32-bit logits: greedy (argmax) and temperature sampling with
-// optional top-k and top-p, one thread block per row, plus a small kernel that edits single logits
-// (presence penalty, banned ids) and one that applies all rules of a request to its row in one pass
-// (penalties over the token history, biases, a mask of allowed ids).
+// optional top-k and top-p, one thread block per row, plus one kernel that applies all rules of a request to its row
+// in one pass (penalties over the token history, biases, banned ids, a mask of allowed ids) and a small one that edits
+// single logits in place (an operator of its own; the sampler uses the rules).
 //
 // Reference parity (the reference samples on the CPU):
 //   greedy       src/scheduler/continuous_batch_engine.cpp:20-62   strict '>' so the lowest index wins ties
